@@ -186,6 +186,90 @@ int b200mm_gqa_decode(const void* q, int64_t q_sb, int64_t q_sh,
                       void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * 8-bit KV cache (no reference counterpart: the engine's cache is 16-bit).
+ * One layer's storage for rows 0.. of a batch, KV heads of D values and a
+ * capacity of S tokens.  Tokens 64 j .. 64 j + 63 of a (row, head) share a
+ * scale, K and V each:
+ *     s = a / 127 (fp32), q = round-half-even(x / s), x' = q s,
+ * with a the largest |x| of the block's tokens so far.  a = 0: s = 0, q = 0;
+ * an infinity or NaN among them: s is not finite, q = 0 and every x' is NaN.
+ *   kq, vq : int8 [*, KV, S, D]     strides (q_sb, q_sh), [S, D] dense
+ *   ks, vs : fp32 [*, KV, S / 64]   strides (s_sb, s_sh), unit inner
+ *   kt, vt : `dtype` [*, KV, 64, D] strides (t_sb, t_sh), [64, D] dense: the
+ *            tokens, as they came, of the block that the row's last append
+ *            ended in (token t in row t % 64)
+ * All zero is the empty cache.  S is a multiple of 64 and at most 2^24; D is a
+ * multiple of 16 and at most 256.  kq, vq, kt, vt and their strides are
+ * 16-byte aligned.
+ *
+ * b200mm_kv8_append: tokens k, v [B, KV, T, D] (strides sb, sh, st, unit
+ *   inner, 16-byte aligned) enter rows 0..B-1 at positions p .. p + T - 1.  p
+ *   is `pos`, or with pos_dev not NULL pos_dev[b * pos_stride] (device int64;
+ *   pos_stride 0: one for all rows, 1: one per row).  A row whose p is
+ *   negative is left as it is; tokens past S are not stored.  p continues the
+ *   row's last append, or lies in the block that it ended in (its tokens from
+ *   p on are then written anew); p = 0 begins a row.  What is stored depends
+ *   on the tokens alone, not on how many came at a time.
+ * b200mm_kv8_expand: k, v [B, KV, L, D] `dtype` (strides o_sb, o_sh, o_st) =
+ *   the values x' of tokens 0..L-1.
+ * b200mm_kv8_decode: one query token per row over the row's tokens,
+ *     out[b, h] = softmax_t(q[b, h] . k'[b, h / g, t] * scale) v'[b, h / g, t],
+ *   t <= p (p as above: the position of the last token attended to, at most
+ *   S - 1), g = H / KV; zeros where p is negative.  q, out: [B, H, D] `dtype`;
+ *   q 16-byte aligned (address and strides).  fp32 softmax and accumulation,
+ *   16-bit products (exact for the 8-bit values; the probabilities keep 11
+ *   bits), one rounding on store.  16-bit types with D = 64 or 128 and g <= 16
+ *   take the split-context kernel; everything else a generic kernel.
+ *   workspace: >= b200mm_kv8_decode_workspace_size bytes (may be 0), 256-byte
+ *   aligned, owned by the stream until the call completes; nothing in it has
+ *   to be initialised, and nothing is kept in it between calls.
+ * b200mm_kv8_step: append of one token per row (k, v [B, KV, D], strides sb,
+ *   sh) at p, then decode over tokens 0..p.
+ */
+typedef struct b200mm_kv8 {
+  int8_t* kq;
+  float* ks;
+  void* kt;
+  int8_t* vq;
+  float* vs;
+  void* vt;
+  int64_t q_sb, q_sh;
+  int64_t s_sb, s_sh;
+  int64_t t_sb, t_sh;
+  int64_t S;
+  int32_t KV, D;
+  int32_t dtype;
+  int32_t reserved;
+} b200mm_kv8;
+
+int b200mm_kv8_append(const b200mm_kv8* cache,
+                      const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                      const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st,
+                      int64_t B, int64_t T,
+                      int64_t pos, const int64_t* pos_dev, int64_t pos_stride, void* stream);
+
+int b200mm_kv8_expand(const b200mm_kv8* cache, void* k, void* v, int64_t o_sb, int64_t o_sh, int64_t o_st,
+                      int64_t B, int64_t L, void* stream);
+
+size_t b200mm_kv8_decode_workspace_size(const b200mm_kv8* cache, int64_t B, int64_t H);
+
+int b200mm_kv8_decode(const b200mm_kv8* cache,
+                      const void* q, int64_t q_sb, int64_t q_sh,
+                      void* out, int64_t o_sb, int64_t o_sh,
+                      int64_t B, int64_t H,
+                      int64_t pos, const int64_t* pos_dev, int64_t pos_stride,
+                      float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+int b200mm_kv8_step(const b200mm_kv8* cache,
+                    const void* q, int64_t q_sb, int64_t q_sh,
+                    const void* k, int64_t k_sb, int64_t k_sh,
+                    const void* v, int64_t v_sb, int64_t v_sh,
+                    void* out, int64_t o_sb, int64_t o_sh,
+                    int64_t B, int64_t H,
+                    int64_t pos, const int64_t* pos_dev, int64_t pos_stride,
+                    float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * MLA latent-cache shapes shared by the two MLA entry points.
  *   B      batch rows served by this call (rows 0..B-1 of the cache)
  *   H      query heads, KV key/value groups (H % KV == 0)

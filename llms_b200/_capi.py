@@ -56,6 +56,30 @@ class PeerOut(ctypes.Structure):
     ]
 
 
+class Kv8(ctypes.Structure):
+    """Mirror of ``b200mm_kv8``."""
+
+    _fields_ = [
+        ("kq", ctypes.c_void_p),
+        ("ks", ctypes.c_void_p),
+        ("kt", ctypes.c_void_p),
+        ("vq", ctypes.c_void_p),
+        ("vs", ctypes.c_void_p),
+        ("vt", ctypes.c_void_p),
+        ("q_sb", ctypes.c_int64),
+        ("q_sh", ctypes.c_int64),
+        ("s_sb", ctypes.c_int64),
+        ("s_sh", ctypes.c_int64),
+        ("t_sb", ctypes.c_int64),
+        ("t_sh", ctypes.c_int64),
+        ("S", ctypes.c_int64),
+        ("KV", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); kept in the order of include/b200mm.h
 SIGNATURES: dict[str, tuple] = {
     "b200mm_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -91,6 +115,26 @@ SIGNATURES: dict[str, tuple] = {
         ctypes.c_int,
         [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_int, _c_p, ctypes.c_size_t, _c_p],
+    ),
+    "b200mm_kv8_append": (
+        ctypes.c_int,
+        [ctypes.POINTER(Kv8), _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_i64, _c_p, _c_i64, _c_p],
+    ),
+    "b200mm_kv8_expand": (
+        ctypes.c_int,
+        [ctypes.POINTER(Kv8), _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p],
+    ),
+    "b200mm_kv8_decode_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(Kv8), _c_i64, _c_i64]),
+    "b200mm_kv8_decode": (
+        ctypes.c_int,
+        [ctypes.POINTER(Kv8), _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64,
+         ctypes.c_float, _c_p, ctypes.c_size_t, _c_p],
+    ),
+    "b200mm_kv8_step": (
+        ctypes.c_int,
+        [ctypes.POINTER(Kv8), _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_p, _c_i64, ctypes.c_float, _c_p, ctypes.c_size_t, _c_p],
     ),
     "b200mm_mla_append": (
         ctypes.c_int,

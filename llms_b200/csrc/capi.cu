@@ -7,6 +7,7 @@
 
 #include <cstdlib>
 #include <string>
+#include "kv8.cuh"
 #include "mla.cuh"
 
 namespace b200mm {
@@ -317,6 +318,125 @@ int b200mm_gqa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* k, 
                   (int)KV, (int)D, L, scale, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
   if (st != B200MM_OK) return st;
   return launch_status();
+}
+
+namespace {
+bool kv8_al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+int kv8_check(const b200mm_kv8* c, int64_t B) {
+  if (!c) return B200MM_ERR_ARG;
+  if (c->dtype != B200MM_F32 && c->dtype != B200MM_F16 && c->dtype != B200MM_BF16) return B200MM_ERR_DTYPE;
+  if (B < 0 || B > 65535 || c->KV < 1 || c->KV > 32767 || c->D < 16 || c->D > 256 || c->D % 16 || c->S < 64 ||
+      c->S > (int64_t(1) << 24) || c->S % 64)
+    return B200MM_ERR_SHAPE;
+  if (!c->kq || !c->ks || !c->kt || !c->vq || !c->vs || !c->vt) return B200MM_ERR_ARG;
+  if (c->q_sh < c->S * c->D || c->q_sb < 0 || c->s_sh < c->S / 64 || c->s_sb < 0 || c->t_sh < 64 * c->D || c->t_sb < 0)
+    return B200MM_ERR_SHAPE;
+  // rows of their own for every batch row
+  if (B > 1 && (c->q_sb < c->S * c->D || c->s_sb < c->S / 64 || c->t_sb < 64 * c->D)) return B200MM_ERR_SHAPE;
+  const int esz = c->dtype == B200MM_F32 ? 4 : 2;
+  if (!kv8_al16(c->kq) || !kv8_al16(c->vq) || !kv8_al16(c->kt) || !kv8_al16(c->vt) || c->q_sb % 16 || c->q_sh % 16 ||
+      (c->t_sb * esz) % 16 || (c->t_sh * esz) % 16)
+    return B200MM_ERR_ALIGN;
+  return B200MM_OK;
+}
+
+int kv8_check_pos(int64_t pos, const int64_t* pos_dev, int64_t pos_stride, int64_t S) {
+  if (pos_stride != 0 && pos_stride != 1) return B200MM_ERR_ARG;
+  if (!pos_dev && (pos < -1 || pos >= S)) return B200MM_ERR_SHAPE;  // a device position is bounded in the kernels
+  return B200MM_OK;
+}
+
+// one of the token tensors of an append: strides in elements
+int kv8_check_tokens(const b200mm_kv8& c, const void* x, int64_t sb, int64_t sh, int64_t st) {
+  if (!x) return B200MM_ERR_ARG;
+  if (sb < 0 || sh < 0 || st < 0) return B200MM_ERR_SHAPE;
+  const int esz = c.dtype == B200MM_F32 ? 4 : 2;
+  if (!kv8_al16(x) || (sb * esz) % 16 || (sh * esz) % 16 || (st * esz) % 16) return B200MM_ERR_ALIGN;
+  return B200MM_OK;
+}
+
+int kv8_check_decode(const b200mm_kv8& c, const void* q, int64_t q_sb, int64_t q_sh, const void* out, int64_t o_sb,
+                     int64_t o_sh, int64_t B, int64_t H, float scale, const void* ws, size_t ws_bytes) {
+  if (H < c.KV || H > 65535 || H % c.KV) return B200MM_ERR_SHAPE;
+  if (!q || !out || !(scale > 0.f)) return B200MM_ERR_ARG;
+  if (q_sb < 0 || q_sh < 0 || o_sb < 0 || o_sh < 0) return B200MM_ERR_SHAPE;
+  const int esz = c.dtype == B200MM_F32 ? 4 : 2;
+  if (!kv8_al16(q) || (q_sb * esz) % 16 || (q_sh * esz) % 16) return B200MM_ERR_ALIGN;
+  if (B == 0) return B200MM_OK;
+  const size_t need = kv8_decode_workspace_bytes(c, (int)B, (int)H);
+  if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255u))) return B200MM_ERR_WORKSPACE;
+  return B200MM_OK;
+}
+}  // namespace
+
+int b200mm_kv8_append(const b200mm_kv8* c, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void* v,
+                      int64_t v_sb, int64_t v_sh, int64_t v_st, int64_t B, int64_t T, int64_t pos,
+                      const int64_t* pos_dev, int64_t pos_stride, void* stream) {
+  int st = kv8_check(c, B);
+  if (st != B200MM_OK) return st;
+  if (T < 0 || T > c->S) return B200MM_ERR_SHAPE;
+  if ((st = kv8_check_pos(pos, pos_dev, pos_stride, c->S)) != B200MM_OK) return st;
+  if (!pos_dev && pos >= 0 && pos + T > c->S) return B200MM_ERR_SHAPE;
+  if ((st = kv8_check_tokens(*c, k, k_sb, k_sh, k_st)) != B200MM_OK) return st;
+  if ((st = kv8_check_tokens(*c, v, v_sb, v_sh, v_st)) != B200MM_OK) return st;
+  if (B == 0 || T == 0) return B200MM_OK;
+  if ((st = check_device()) != B200MM_OK) return st;
+  st = kv8_append(*c, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, (int)B, T, Kv8Pos{pos_dev, pos, (int)pos_stride},
+                  static_cast<cudaStream_t>(stream));
+  return st != B200MM_OK ? st : launch_status();
+}
+
+int b200mm_kv8_expand(const b200mm_kv8* c, void* k, void* v, int64_t o_sb, int64_t o_sh, int64_t o_st, int64_t B,
+                      int64_t L, void* stream) {
+  int st = kv8_check(c, B);
+  if (st != B200MM_OK) return st;
+  if (L < 0 || L > c->S || o_st < c->D || o_sh < 0 || o_sb < 0) return B200MM_ERR_SHAPE;
+  if ((st = kv8_check_tokens(*c, k, o_sb, o_sh, o_st)) != B200MM_OK) return st;
+  if ((st = kv8_check_tokens(*c, v, o_sb, o_sh, o_st)) != B200MM_OK) return st;
+  if (B == 0 || L == 0) return B200MM_OK;
+  if ((st = check_device()) != B200MM_OK) return st;
+  st = kv8_expand(*c, k, v, o_sb, o_sh, o_st, (int)B, L, static_cast<cudaStream_t>(stream));
+  return st != B200MM_OK ? st : launch_status();
+}
+
+size_t b200mm_kv8_decode_workspace_size(const b200mm_kv8* c, int64_t B, int64_t H) {
+  if (kv8_check(c, B) != B200MM_OK || B == 0 || H < c->KV || H > 65535 || H % c->KV) return 0;
+  return kv8_decode_workspace_bytes(*c, (int)B, (int)H);
+}
+
+int b200mm_kv8_decode(const b200mm_kv8* c, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb,
+                      int64_t o_sh, int64_t B, int64_t H, int64_t pos, const int64_t* pos_dev, int64_t pos_stride,
+                      float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = kv8_check(c, B);
+  if (st != B200MM_OK) return st;
+  if ((st = kv8_check_pos(pos, pos_dev, pos_stride, c->S)) != B200MM_OK) return st;
+  st = kv8_check_decode(*c, q, q_sb, q_sh, out, o_sb, o_sh, B, H, scale, workspace, workspace_bytes);
+  if (st != B200MM_OK || B == 0) return st;
+  if ((st = check_device()) != B200MM_OK) return st;
+  st = kv8_decode(*c, q, q_sb, q_sh, out, o_sb, o_sh, (int)B, (int)H, Kv8Pos{pos_dev, pos, (int)pos_stride}, scale,
+                  workspace, static_cast<cudaStream_t>(stream));
+  return st != B200MM_OK ? st : launch_status();
+}
+
+int b200mm_kv8_step(const b200mm_kv8* c, const void* q, int64_t q_sb, int64_t q_sh, const void* k, int64_t k_sb,
+                    int64_t k_sh, const void* v, int64_t v_sb, int64_t v_sh, void* out, int64_t o_sb, int64_t o_sh,
+                    int64_t B, int64_t H, int64_t pos, const int64_t* pos_dev, int64_t pos_stride, float scale,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  int st = kv8_check(c, B);
+  if (st != B200MM_OK) return st;
+  if ((st = kv8_check_pos(pos, pos_dev, pos_stride, c->S)) != B200MM_OK) return st;
+  if ((st = kv8_check_tokens(*c, k, k_sb, k_sh, 0)) != B200MM_OK) return st;
+  if ((st = kv8_check_tokens(*c, v, v_sb, v_sh, 0)) != B200MM_OK) return st;
+  st = kv8_check_decode(*c, q, q_sb, q_sh, out, o_sb, o_sh, B, H, scale, workspace, workspace_bytes);
+  if (st != B200MM_OK || B == 0) return st;
+  if ((st = check_device()) != B200MM_OK) return st;
+  const Kv8Pos p{pos_dev, pos, (int)pos_stride};
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  st = kv8_append(*c, k, k_sb, k_sh, 0, v, v_sb, v_sh, 0, (int)B, 1, p, s);
+  if (st != B200MM_OK) return st;
+  st = kv8_decode(*c, q, q_sb, q_sh, out, o_sb, o_sh, (int)B, (int)H, p, scale, workspace, s);
+  return st != B200MM_OK ? st : launch_status();
 }
 
 int b200mm_mla_append(const b200mm_mla_shape* shape, const void* c_kv, int64_t c_sb, int64_t c_st,

@@ -1,0 +1,238 @@
+// 8-bit KV cache: tokens in (append) and out again (expand).
+//
+// Block j of a (row, head) holds tokens 64 j .. 64 j + 63.  Over the tokens
+// that are there, with a = max |x|:
+//     s = fl32(a / 127),   q = round-half-even(x / s),   x' = q s.
+// The rounding decides on the exact quotient, not on a rounded one: with
+// t = rint(x * fl(1/s)), which is off by at most one, the remainder x - t s is
+// exact in one fma and is compared with s / 2.  So the stored bits are a
+// function of the tokens alone.  a == 0 gives s = 0, q = 0; an infinity or NaN
+// among the tokens gives a scale that is not finite and q = 0, so that every
+// value of the block reads as NaN.
+//
+// The scale of an open block moves as it fills.  Rescaling 8-bit values would
+// round a token again each time, so the tokens of the block that the last
+// append ended in are also kept as they came (the tail, 64 rows), and when the
+// scale moves the block is quantised again from them: token by token gives the
+// same bits as all at once, and writing a token again gives what writing it
+// once gives.
+//
+// append: one CTA per (block, head, row) and K / V.  A CTA keeps its block (64
+// tokens) in registers between the maximum and the rounding, so each token is
+// read once.  Single tokens read the block's earlier tokens (at most 63 rows
+// from the tail) and write one row of 8 bits while the scale stands.
+// expand: 16 values per thread.  Both are streams, bound by HBM at length and
+// by one launch for single tokens.
+#include "kv8.cuh"
+
+namespace b200mm {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendArgs {
+  b200mm_kv8 c;
+  const void* src[2];
+  int64_t sb[2], sh[2], st[2];
+  int64_t T;
+  Kv8Pos pos;
+};
+
+__device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
+
+// round-half-even(x / s) for |x| <= 127 s (1 + 2^-24), s normal, inv = fl(1 / s)
+__device__ __forceinline__ int quantize(float x, float s, float inv) {
+  float t = rintf(x * inv);
+  const float d2 = 2.f * fmaf(-t, s, x);  // exact
+  const bool odd = (__float2int_rn(t) & 1) != 0;
+  if (d2 > s || (odd && d2 == s)) t += 1.f;
+  if (d2 < -s || (odd && d2 == -s)) t -= 1.f;
+  return __float2int_rn(t);
+}
+
+// The same for a subnormal scale, whose reciprocal may overflow: the quotient
+// in 64 bits (53 bits hold it to far less than its distance from a border:
+// x and s have at most 24 bits).
+__device__ __noinline__ int quantize_small(float x, float s) { return (int)rint((double)x / (double)s); }
+
+// Quantise block `blk` of one (row, head): rows [0, r0) come from the tail,
+// rows [r0, r1) from `src` (row r0's address), the rest is not there.
+template <typename T, int NC>
+__device__ void do_block(const T* src, int64_t src_st, T* tail, int8_t* qdst, float* sdst, int D, int r0, int r1,
+                         bool write_tail, uint32_t* red) {
+  constexpr int V = 16 / sizeof(T);  // elements per 16-byte chunk
+  const int cpr = D / V;             // chunks per row
+  const int total = r1 * cpr;
+  uint4 x[NC];
+  uint32_t mx = 0;
+  const uint32_t s_old = __float_as_uint(*sdst);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int idx = threadIdx.x + i * kThreads;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (idx < total) {
+      const int row = idx / cpr, c = idx - row * cpr;
+      const T* p = row < r0 ? tail + (int64_t)row * D : src + (int64_t)(row - r0) * src_st;
+      x[i] = *reinterpret_cast<const uint4*>(p + c * V);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    float f[V];
+    Chunk<T>::unpack(x[i], f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) mx = max(mx, abs_bits(f[e]));  // ordered as the values; NaN above infinity
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mx;
+  __syncthreads();  // (also: every thread has read s_old)
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) mx = max(mx, red[w]);
+  const float s = __fdiv_rn(__uint_as_float(mx), 127.f);
+  const bool finite = mx < 0x7f800000u, some = s > 0.f;
+  const bool all_rows = __float_as_uint(s) != s_old;
+  const float inv = __frcp_rn(s);
+  const bool normal = s >= 1.17549435e-38f;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int idx = threadIdx.x + i * kThreads;
+    if (idx >= total) continue;
+    const int row = idx / cpr, c = idx - row * cpr;
+    if (write_tail && row >= r0) *reinterpret_cast<uint4*>(tail + (int64_t)row * D + c * V) = x[i];
+    if (row < r0 && !all_rows) continue;
+    float f[V];
+    Chunk<T>::unpack(x[i], f);
+    uint32_t o[V / 4];
+#pragma unroll
+    for (int w = 0; w < V / 4; ++w) {
+      uint32_t word = 0;
+      if (finite && some) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = f[4 * w + e];
+          const int q = normal ? quantize(y, s, inv) : quantize_small(y, s);
+          word |= (uint32_t)(q & 255) << (8 * e);
+        }
+      }
+      o[w] = word;
+    }
+    int8_t* dst = qdst + (int64_t)row * D + c * V;
+    if constexpr (V == 8)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+    else
+      *reinterpret_cast<uint32_t*>(dst) = o[0];
+  }
+  if (threadIdx.x == 0) *sdst = s;
+}
+
+template <typename T, int NC>
+__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
+  __shared__ uint32_t red[kThreads / 32];
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1;
+  const int64_t p0 = a.pos(b);
+  if (p0 < 0 || p0 >= a.c.S) return;  // a row that is not there, or past the capacity
+  const int64_t p1 = p0 + a.T < a.c.S ? p0 + a.T : a.c.S;
+  const int64_t first = p0 / kKv8Block, last = (p1 - 1) / kKv8Block;
+  const int D = a.c.D, r0 = (int)(p0 % kKv8Block);
+  const T* src = static_cast<const T*>(a.src[which]) + (int64_t)b * a.sb[which] + (int64_t)h * a.sh[which];
+  T* tail = static_cast<T*>(which ? a.c.vt : a.c.kt) + (int64_t)b * a.c.t_sb + (int64_t)h * a.c.t_sh;
+  int8_t* q = (which ? a.c.vq : a.c.kq) + (int64_t)b * a.c.q_sb + (int64_t)h * a.c.q_sh;
+  float* s = (which ? a.c.vs : a.c.ks) + (int64_t)b * a.c.s_sb + (int64_t)h * a.c.s_sh;
+  auto run = [&](int64_t blk) {
+    const int64_t t0 = blk * kKv8Block;
+    const int lo = blk == first ? r0 : 0;
+    const int hi = (int)(p1 - t0 < kKv8Block ? p1 - t0 : kKv8Block);
+    do_block<T, NC>(src + (t0 + lo - p0) * a.st[which], a.st[which], tail, q + t0 * D, s + blk, D, lo, hi, blk == last,
+                    red);
+  };
+  const int64_t blk = first + blockIdx.x;
+  if (blk > last) return;
+  // a first block that reads the tail and a last block that writes it are one CTA's, in this order
+  const bool both = r0 > 0 && last > first;
+  if (both && blk == last) return;
+  run(blk);
+  if (both && blk == first) {
+    __syncthreads();
+    run(last);
+  }
+}
+
+struct ExpandArgs {
+  b200mm_kv8 c;
+  void* dst[2];
+  int64_t o_sb, o_sh, o_st;
+  int64_t L;
+};
+
+// 16 values of one token per thread.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) kv8_expand_kernel(const __grid_constant__ ExpandArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1;
+  const int cpr = a.c.D / 16;
+  const int64_t n = a.L * cpr;
+  const int8_t* q = (which ? a.c.vq : a.c.kq) + (int64_t)b * a.c.q_sb + (int64_t)h * a.c.q_sh;
+  const float* s = (which ? a.c.vs : a.c.ks) + (int64_t)b * a.c.s_sb + (int64_t)h * a.c.s_sh;
+  T* dst = static_cast<T*>(a.dst[which]) + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    const int64_t t = i / cpr;
+    const int c = (int)(i - t * cpr);
+    float f[16];
+    Chunk<int8_t>::unpack(__ldcs(reinterpret_cast<const uint4*>(q + t * a.c.D + 16 * c)), f);
+    const float sc = s[t / kKv8Block];
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int w = 0; w < 16 / V; ++w) {
+      T o[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = from_f<T>(f[w * V + e] * sc);
+      *reinterpret_cast<uint4*>(dst + t * a.o_st + 16 * c + w * V) = *reinterpret_cast<const uint4*>(o);
+    }
+  }
+}
+
+template <typename T>
+int append_t(const AppendArgs& a, int B, cudaStream_t st) {
+  // blocks that T tokens touch, wherever they start
+  const int64_t nb = (a.T + kKv8Block - 2) / kKv8Block + 1;
+  const int64_t cap = a.c.S / kKv8Block;
+  const dim3 grid((unsigned)(nb < cap ? nb : cap), 2 * a.c.KV, B);
+  // 64 D elements, 16 bytes per thread and step
+  const bool small = (size_t)kKv8Block * a.c.D * sizeof(T) <= (size_t)kThreads * 16 * 4;
+  const cudaError_t e = small ? launch_pdl(kv8_append_kernel<T, 4>, grid, dim3(kThreads), 0, st, a)
+                              : launch_pdl(kv8_append_kernel<T, 16>, grid, dim3(kThreads), 0, st, a);
+  return e == cudaSuccess ? B200MM_OK : B200MM_ERR_LAUNCH;
+}
+
+template <typename T>
+int expand_t(const ExpandArgs& a, int B, cudaStream_t st) {
+  const int64_t n = a.L * (a.c.D / 16);
+  const int64_t want = (n + kThreads - 1) / kThreads;
+  const dim3 grid((unsigned)(want < 4096 ? want : 4096), 2 * a.c.KV, B);
+  return launch_pdl(kv8_expand_kernel<T>, grid, dim3(kThreads), 0, st, a) == cudaSuccess ? B200MM_OK
+                                                                                       : B200MM_ERR_LAUNCH;
+}
+
+}  // namespace
+
+int kv8_append(const b200mm_kv8& c, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void* v,
+               int64_t v_sb, int64_t v_sh, int64_t v_st, int B, int64_t T, Kv8Pos pos, cudaStream_t st) {
+  const AppendArgs a{c, {k, v}, {k_sb, v_sb}, {k_sh, v_sh}, {k_st, v_st}, T, pos};
+  if (c.dtype == B200MM_BF16) return append_t<__nv_bfloat16>(a, B, st);
+  if (c.dtype == B200MM_F16) return append_t<__half>(a, B, st);
+  return append_t<float>(a, B, st);
+}
+
+int kv8_expand(const b200mm_kv8& c, void* k, void* v, int64_t o_sb, int64_t o_sh, int64_t o_st, int B, int64_t L,
+               cudaStream_t st) {
+  const ExpandArgs a{c, {k, v}, o_sb, o_sh, o_st, L};
+  if (c.dtype == B200MM_BF16) return expand_t<__nv_bfloat16>(a, B, st);
+  if (c.dtype == B200MM_F16) return expand_t<__half>(a, B, st);
+  return expand_t<float>(a, B, st);
+}
+
+}  // namespace b200mm

@@ -8,6 +8,7 @@ decode attention op.
 from .decode_attn import apply_decode_attn, b200_decode_attn
 from .fused_ffn import TritonFFN, triton_fused_gate_up_silu
 from .fused_qkv import TritonAttention, triton_fused_qkv
+from .kv8 import Int8KV, Int8KVCache, int8_kv_append, int8_kv_decode_attn, int8_kv_expand, int8_kv_step
 from .linear import B200Linear, Int8Linear, b200_linear, int8_linear
 from .quant import (
     Int8Attention,
@@ -20,6 +21,12 @@ from .quant import (
 from .swap import apply_int8_kernels, apply_linear_kernels, apply_triton_kernels, prewarm_triton_kernels
 
 __all__ = [
+    "Int8KV",
+    "Int8KVCache",
+    "int8_kv_append",
+    "int8_kv_decode_attn",
+    "int8_kv_expand",
+    "int8_kv_step",
     "apply_decode_attn",
     "b200_decode_attn",
     "B200Linear",

@@ -1,0 +1,128 @@
+"""Refusals of the 8-bit KV cache calls, on the host: nothing is launched."""
+
+import ctypes
+
+import pytest
+import torch
+
+from llms_b200 import _capi
+from llms_b200.kernels import Int8KV, Int8KVCache, int8_kv_append, int8_kv_decode_attn, int8_kv_expand, int8_kv_step
+
+
+def _kv(rows=2, KV=2, S=128, D=64, dtype=torch.bfloat16):
+    return Int8KV.alloc(rows=rows, num_kv_heads=KV, max_seq_len=S, head_dim=D, dtype=dtype, device="cpu")
+
+
+def test_alloc_rounds_the_capacity_up():
+    assert _kv(S=1).capacity == 64 and _kv(S=64).capacity == 64 and _kv(S=65).capacity == 128
+
+
+@pytest.mark.parametrize("change", [
+    {"kq": torch.zeros(2, 2, 128, 64), "vq": torch.zeros(2, 2, 128, 64)},                       # not int8
+    {"kq": torch.zeros(2, 2, 100, 64, dtype=torch.int8), "vq": torch.zeros(2, 2, 100, 64, dtype=torch.int8)},
+    {"kq": torch.zeros(2, 2, 128, 72, dtype=torch.int8), "vq": torch.zeros(2, 2, 128, 72, dtype=torch.int8)},
+    {"vs": torch.zeros(2, 2, 3)},
+    {"ks": torch.zeros(2, 2, 1), "vs": torch.zeros(2, 2, 1)},
+    {"ks": torch.zeros(2, 2, 2, dtype=torch.float64), "vs": torch.zeros(2, 2, 2, dtype=torch.float64)},
+    {"kt": torch.zeros(2, 2, 32, 64), "vt": torch.zeros(2, 2, 32, 64)},
+    {"kt": torch.zeros(2, 2, 64, 64, dtype=torch.float64), "vt": torch.zeros(2, 2, 64, 64, dtype=torch.float64)},
+    {"kq": torch.zeros(2, 2, 64, 128, dtype=torch.int8).transpose(2, 3),
+     "vq": torch.zeros(2, 2, 64, 128, dtype=torch.int8).transpose(2, 3)},                      # tokens not contiguous
+])
+def test_storage_refused(change):
+    kv = _kv()
+    parts = {n: getattr(kv, n) for n in ("kq", "ks", "kt", "vq", "vs", "vt")}
+    with pytest.raises(ValueError):
+        Int8KV(**{**parts, **change})
+
+
+def test_calls_refused():
+    kv = _kv()
+    q, k = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        int8_kv_append(kv, k, k, 0)  # a CPU cache
+    with pytest.raises(RuntimeError):
+        int8_kv_decode_attn(q, kv, 0, scale=0.1)
+    with pytest.raises(RuntimeError):
+        int8_kv_expand(kv, 5)
+    for bad in (k[:, :1], k[..., :32], k.float(), k[:, :, 0]):
+        with pytest.raises(ValueError):
+            int8_kv_append(kv, bad, bad, 0)
+    with pytest.raises(ValueError):
+        int8_kv_append(kv, k, k.expand(2, 2, 2, 64), 0)
+    with pytest.raises(ValueError):
+        int8_kv_append(kv, torch.zeros(3, 2, 1, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 1, 64, dtype=torch.bfloat16), 0)
+    for bad in (q[:, :3], q[..., :32], q.half(), q.expand(2, 4, 2, 64), q[0]):
+        with pytest.raises(ValueError):
+            int8_kv_decode_attn(bad, kv, 0, scale=0.1)
+    with pytest.raises(ValueError):
+        int8_kv_expand(kv, 129)
+    with pytest.raises(ValueError):
+        int8_kv_expand(kv, 1, batch=3)
+
+
+def _c_cache(**kw):
+    f = dict(kq=4096, ks=4096, kt=4096, vq=4096, vs=4096, vt=4096, q_sb=2 * 128 * 64, q_sh=128 * 64, s_sb=4, s_sh=2,
+             t_sb=2 * 64 * 64, t_sh=64 * 64, S=128, KV=2, D=64, dtype=2, reserved=0)
+    f.update(kw)
+    return _capi.Kv8(**f)
+
+
+OK, SHAPE, ALIGN, DTYPE, ARG, WORKSPACE = 0, 1, 2, 3, 5, 6
+
+
+def _append(c, B=2, T=1, pos=0, stride=0, p=4096, ld=64):
+    return _capi.lib.b200mm_kv8_append(ctypes.byref(c), p, 2 * ld, ld, ld, p, 2 * ld, ld, ld, B, T, pos, None, stride, None)
+
+
+def _decode(c, B=2, H=4, pos=0, stride=0, scale=0.1, ws=4096, n=1 << 30, q=4096):
+    return _capi.lib.b200mm_kv8_decode(ctypes.byref(c), q, H * 64, 64, 4096, H * 64, 64, B, H, pos, None, stride, scale,
+                                       ws, n, None)
+
+
+def test_c_entry_points_refuse_before_any_launch():
+    before = _capi.launch_count()
+    for bad, code in (({"dtype": 7}, DTYPE), ({"S": 100}, SHAPE), ({"S": 0}, SHAPE), ({"S": (1 << 24) + 64, "q_sh": 1 << 40}, SHAPE),
+                      ({"D": 8}, SHAPE), ({"D": 272}, SHAPE), ({"D": 40}, SHAPE), ({"KV": 0}, SHAPE), ({"ks": None}, ARG),
+                      ({"vt": None}, ARG), ({"q_sh": 64}, SHAPE), ({"q_sb": 0}, SHAPE), ({"t_sb": 0}, SHAPE), ({"s_sh": 1}, SHAPE),
+                      ({"kq": 4097}, ALIGN), ({"q_sb": 2 * 128 * 64 + 8}, ALIGN), ({"t_sh": 64 * 64 + 4}, ALIGN)):
+        c = _c_cache(**bad)
+        assert _append(c) == code, bad
+        assert _decode(c) == code, bad
+        assert _capi.lib.b200mm_kv8_decode_workspace_size(ctypes.byref(c), 2, 4) == 0, bad
+    c = _c_cache()
+    assert _append(c, B=-1) == SHAPE and _append(c, T=-1) == SHAPE and _append(c, T=129) == SHAPE
+    assert _append(c, pos=128) == SHAPE and _append(c, pos=127, T=2) == SHAPE and _append(c, pos=-2) == SHAPE
+    assert _append(c, stride=2) == ARG and _append(c, p=None) == ARG and _append(c, p=4100) == ALIGN and _append(c, ld=68) == ALIGN
+    assert _append(c, B=0) == OK and _append(c, T=0) == OK
+    assert _decode(c, H=3) == SHAPE and _decode(c, H=0) == SHAPE and _decode(c, pos=128) == SHAPE
+    assert _decode(c, scale=0.0) == ARG and _decode(c, scale=float("nan")) == ARG and _decode(c, q=None) == ARG
+    assert _decode(c, q=4104) == ALIGN
+    assert _decode(c, ws=None) == WORKSPACE and _decode(c, n=16) == WORKSPACE and _decode(c, ws=4096 + 16) == WORKSPACE
+    assert _decode(c, B=0) == OK
+    assert _capi.lib.b200mm_kv8_append(None, None, 0, 0, 0, None, 0, 0, 0, 1, 1, 0, None, 0, None) == ARG
+    assert _capi.launch_count() == before
+
+
+def test_rewind_takes_the_open_block_from_its_8_bit_values():
+    kv = _kv(rows=1, KV=1, S=256)
+    kv.length = 200
+    kv.kq.copy_(torch.arange(256 * 64).remainder(255).sub(127).view(1, 1, 256, 64))
+    kv.ks.fill_(0.5)
+    kv.kt.fill_(7)
+    kv.rewind(195)  # inside the last block: its tokens are there
+    assert kv.length == 195 and (kv.kt == 7).all()
+    kv.rewind(70)
+    assert torch.equal(kv.kt[0, 0, :6], (kv.kq[0, 0, 64:70].float() * 0.5).bfloat16()) and (kv.kt[0, 0, 6:] == 7).all()
+    with pytest.raises(ValueError):
+        kv.rewind(71)
+
+
+def test_model_cache_counts_and_seeks():
+    c = Int8KVCache.alloc(num_layers=2, max_batch=1, num_kv_heads=1, max_seq_len=100, head_dim=64, dtype=torch.float16, device="cpu")
+    assert c.capacity == 128 and c.cur_len == 0
+    c.cur_len = 90
+    c.seek(64)
+    assert c.cur_len == 64 and [x.length for x in c.layers] == [64, 64]
+    with pytest.raises(ValueError):
+        c.seek(65)
