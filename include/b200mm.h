@@ -270,6 +270,24 @@ int b200mm_kv8_step(const b200mm_kv8* cache,
                     float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Log probabilities of given tokens under rows of logits (no reference
+ * counterpart: the engine's sampler, engine/sampler.py, takes the argmax only):
+ *   logprob[m] = x[m, tokens[m]] - lse(x[m, :]),
+ *   entropy[m] = -sum_i p_i log p_i (natural logarithms),
+ *   top_ids[m, 0..top), top_logprobs[m, 0..top): the largest logits in
+ *   descending order, equal ones by ascending index, and their log probabilities.
+ *   x : [M, V] `dtype`, row stride ldx (no alignment asked for); tokens int64
+ *   [M]; logprob, entropy fp32 [M]; top_ids int64 and top_logprobs fp32
+ *   [M, top] dense, may be NULL when top == 0.  0 <= top <= min(V, 64).
+ * -infinity logits (ruled-out tokens) count as probability 0.  A row with a
+ * NaN or +infinity, or with nothing but -infinity, has NaN numbers; NaN ranks
+ * above every value.  A token outside [0, V) has a NaN log probability.
+ */
+int b200mm_token_logprobs(const void* x, int64_t ldx, const int64_t* tokens,
+                          float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs,
+                          int64_t M, int64_t V, int64_t top, int dtype, void* stream);
+
+/*
  * MLA latent-cache shapes shared by the two MLA entry points.
  *   B      batch rows served by this call (rows 0..B-1 of the cache)
  *   H      query heads, KV key/value groups (H % KV == 0)

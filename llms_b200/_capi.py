@@ -136,6 +136,10 @@ SIGNATURES: dict[str, tuple] = {
         [ctypes.POINTER(Kv8), _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_p, _c_i64, ctypes.c_float, _c_p, ctypes.c_size_t, _c_p],
     ),
+    "b200mm_token_logprobs": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p],
+    ),
     "b200mm_mla_append": (
         ctypes.c_int,
         [ctypes.POINTER(MlaShape), _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p,

@@ -8,6 +8,7 @@
 #include <cstdlib>
 #include <string>
 #include "kv8.cuh"
+#include "logprobs.cuh"
 #include "mla.cuh"
 
 namespace b200mm {
@@ -436,6 +437,22 @@ int b200mm_kv8_step(const b200mm_kv8* c, const void* q, int64_t q_sb, int64_t q_
   st = kv8_append(*c, k, k_sb, k_sh, 0, v, v_sb, v_sh, 0, (int)B, 1, p, s);
   if (st != B200MM_OK) return st;
   st = kv8_decode(*c, q, q_sb, q_sh, out, o_sb, o_sh, (int)B, (int)H, p, scale, workspace, s);
+  return st != B200MM_OK ? st : launch_status();
+}
+
+int b200mm_token_logprobs(const void* x, int64_t ldx, const int64_t* tokens, float* logprob, float* entropy,
+                          int64_t* top_ids, float* top_logprobs, int64_t M, int64_t V, int64_t top, int dtype,
+                          void* stream) {
+  if (dtype != B200MM_F32 && dtype != B200MM_F16 && dtype != B200MM_BF16) return B200MM_ERR_DTYPE;
+  if (M < 0 || M >= (int64_t(1) << 27) || V < 1 || V >= (int64_t(1) << 31) - 64 || ldx < V) return B200MM_ERR_SHAPE;
+  if (top < 0 || top > V || top > kLogprobsMaxTop) return B200MM_ERR_SHAPE;
+  if (M == 0) return B200MM_OK;
+  if (!x || !tokens || !logprob || !entropy || (top > 0 && (!top_ids || !top_logprobs))) return B200MM_ERR_ARG;
+  if ((uintptr_t)x % (dtype == B200MM_F32 ? 4 : 2)) return B200MM_ERR_ALIGN;
+  int st = check_device();
+  if (st != B200MM_OK) return st;
+  const LogprobsArgs a{x, ldx, tokens, logprob, entropy, top_ids, top_logprobs, M, (int)V, (int)top};
+  st = logprobs_launch(a, dtype, static_cast<cudaStream_t>(stream));
   return st != B200MM_OK ? st : launch_status();
 }
 

@@ -1,0 +1,417 @@
+// Log probabilities of given tokens, entropy and top alternatives of logit rows:
+//   lse = log sum_i e^x_i,  logprob = x[token] - lse,  H = lse - sum_i p_i x_i,
+//   top: the largest x_i in descending order, ties by ascending index.
+//
+// A row is read once, 16 bytes per lane and four loads at a time.  Each thread
+// keeps, over its share of the row, the maximum m, l = sum e^(x - m) and
+// e = sum e^(x - m) (x - m) in fp32, rescaled once per four loads; then
+// lse = m + log l and H = log l - e / l.
+//
+// Top alternatives: 128 groups of threads each know the largest value of their
+// shares.  The k-th largest of these is a bound that at least k elements
+// reach, and only groups that reach it hold any: their shares are read again
+// (a few KB of L2 for k = 20 of 150,000), the elements that reach the bound are
+// collected and ranked by counting.  No sort, and no second pass over the row.
+// Where more elements reach the bound than are kept (a row whose k-th value is
+// the -infinity of a masked vocabulary, or all logits the same), the ones
+// above it are collected and the lowest indices among the equal ones follow in
+// a scan that ends as soon as there are enough.  Rows that defeat this too
+// (thousands above the bound in fewer than k groups) and rows with NaN are
+// searched once per alternative.
+//
+// A cluster of up to 16 CTAs shares a row when there are few rows; sums and
+// alternatives meet in the first CTA through distributed shared memory, so a
+// call is one launch without a workspace.
+#include "logprobs.cuh"
+
+namespace b200mm {
+
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kGroups = 128;              // groups of kThreads / kGroups neighbouring threads
+constexpr int kPer = kThreads / kGroups;
+constexpr int kCand = 2048;               // elements collected at once
+constexpr int kMaxCluster = 16;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFar = -1000.f;           // e^-1000 = 0: stands for -infinity where 0 * x has to be 0
+static_assert(kLogprobsMaxTop <= kGroups, "the bound is one of the groups' largest values");
+
+// Larger key: larger value (NaN above all, -0 and 0 the same), then smaller index.  0: none.
+__device__ __forceinline__ uint32_t value_key(float x) {
+  if (x != x) return 0xfffffffeu;  // (no key is all ones)
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t make_key(float x, uint32_t i) { return ((uint64_t)value_key(x) << 32) | (uint32_t)~i; }
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  return __uint_as_float((b & 0x80000000u) ? b ^ 0x80000000u : ~b);  // (NaN's key reads as a NaN)
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Sums {
+  float m, l, e;
+};
+// max(d, kFar), NaN kept
+__device__ __forceinline__ float near(float d) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(d), "f"(kFar));
+  return y;
+}
+// The reference of a maximum: itself, or 0 where there is nothing but -infinity yet.
+__device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
+// `s` with its maximum raised to at least `m`
+__device__ __forceinline__ void raise(Sums& s, float m) {
+  const float mn = fmaxf(s.m, m);
+  const float d = fmaxf(s.m - ref_of(mn), kFar), f = ex2(d * kLog2e);
+  s.e = (s.e + s.l * d) * f;
+  s.l *= f;
+  s.m = mn;
+}
+__device__ __forceinline__ void add(Sums& s, float x, float ref) {
+  // (x - ref before the factor: logits near the type's limits do not overflow)
+  const float d = near(x - ref), p = ex2(d * kLog2e);
+  s.l += p;
+  s.e = fmaf(p, d, s.e);
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+  raise(a, b.m);
+  raise(b, a.m);
+  return Sums{a.m, a.l + b.l, a.e + b.e};
+}
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr uint32_t kLowest = 0xff800000u;  // -infinity
+  __device__ __forceinline__ static float max4(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr uint32_t kLowest = 0xff80ff80u;
+  __device__ __forceinline__ static float max4(const uint4& v) {
+    auto h = [](const uint32_t& w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
+    return fmaxf(f.x, f.y);
+  }
+};
+template <> struct Vec<__half> {
+  static constexpr uint32_t kLowest = 0xfc00fc00u;
+  __device__ __forceinline__ static float max4(const uint4& v) {
+    auto h = [](const uint32_t& w) { return *reinterpret_cast<const __half2*>(&w); };
+    const float2 f = __half22float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
+    return fmaxf(f.x, f.y);
+  }
+};
+
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsArgs a, const int C) {
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr int U = 4;  // loads in flight per thread
+  __shared__ uint64_t cand[kCand];
+  __shared__ uint64_t list[kLogprobsMaxTop];
+  __shared__ uint64_t lists[kMaxCluster][kLogprobsMaxTop];  // of every CTA (first CTA only)
+  __shared__ float4 all[kMaxCluster];  // the CTAs' m, l, e
+  __shared__ Sums wsum[kWarps];
+  __shared__ uint64_t wkey[kWarps];
+  __shared__ int wcount[kWarps];
+  __shared__ float gbest[kGroups];
+  __shared__ int glist[kGroups];
+  __shared__ float bound;
+  __shared__ int ncand, ngroups;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = C > 1 ? (int)cluster_rank() : 0;
+  const int64_t row = blockIdx.x / C;
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const int V = a.V, top = a.top;
+  pdl_trigger();
+  pdl_wait();
+
+  // the row: `head` elements up to a 16-byte boundary, nv vectors, a tail; the
+  // first CTA's first threads take the single elements
+  const int off = (int)(((uintptr_t)x & 15u) / sizeof(T));
+  const int head = off ? min(V, VEC - off) : 0;
+  const int nv = (V - head) / VEC;
+  const int tail0 = head + nv * VEC;
+  const T* xv = x + head;
+  const int step = C * kThreads;
+  const int v0 = rank * kThreads + tid;
+  auto vec_at = [&](int v) { return *reinterpret_cast<const uint4*>(xv + (int64_t)v * VEC); };
+  auto unpack = [&](const uint4& v, float* f) { Chunk<T>::unpack(v, f); };
+  const bool has_head = rank == 0 && tid < head, has_tail = rank == 0 && tid < V - tail0;
+
+  // ---- the stream ----
+  Sums s{-INFINITY, 0.f, 0.f};
+  float best = -INFINITY;
+  for (int v = v0; v < nv; v += U * step) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w[u] = make_uint4(Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest);
+      if (v + u * step < nv) w[u] = vec_at(v + u * step);
+    }
+    float mx = Vec<T>::max4(w[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) mx = fmaxf(mx, Vec<T>::max4(w[u]));
+    best = fmaxf(best, mx);
+    raise(s, mx);
+    const float ref = ref_of(s.m);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[VEC];
+      unpack(w[u], f);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) add(s, f[i], ref);
+    }
+  }
+  auto single = [&](int i) {
+    const float f = to_f<T>(x[i]);
+    best = fmaxf(best, f);
+    raise(s, f);
+    add(s, f, ref_of(s.m));
+  };
+  if (has_head) single(tid);
+  if (has_tail) single(tail0 + tid);
+
+  Sums t = s;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    t = join(t, Sums{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.l, o),
+                     __shfl_xor_sync(0xffffffffu, t.e, o)});
+  if (lane == 0) wsum[warp] = t;
+  if (top > 0) {
+    float g = best;
+#pragma unroll
+    for (int o = 1; o < kPer; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (tid % kPer == 0) gbest[tid / kPer] = g;
+    if (tid < kLogprobsMaxTop) list[tid] = 0;
+  }
+  __syncthreads();
+  t = wsum[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) t = join(t, wsum[w]);
+
+  // ---- the CTA's alternatives, in order, to list[0 .. top) ----
+  if (top > 0) {
+    if (tid < kGroups) {
+      const float g = gbest[tid];
+      int r = 0;
+      for (int i = 0; i < kGroups; ++i) r += gbest[i] > g || (gbest[i] == g && i < tid);
+      if (r == top - 1) bound = g;
+    }
+    if (tid == 0) ncand = ngroups = 0;
+    __syncthreads();
+    const float tau = bound;
+    if (tid < kGroups && gbest[tid] >= tau) glist[atomicAdd(&ngroups, 1)] = tid;
+    __syncthreads();
+    // elements of the listed groups that reach the bound (`strict`: that lie above it)
+    auto collect = [&](bool strict) {
+      auto offer = [&](float f, int i) {
+        if (strict ? f > tau : f >= tau) {
+          const int at = atomicAdd(&ncand, 1);
+          if (at < kCand) cand[at] = make_key(f, (uint32_t)i);
+        }
+      };
+      const int iters = (nv - rank * kThreads + step - 1) / step;  // of the CTA's first thread
+      const int items = ngroups * kPer * max(iters, 0);
+      for (int i = tid; i < items; i += kThreads) {
+        const int sub = i % kPer, gi = (i / kPer) % ngroups, it = i / (kPer * ngroups);
+        const int v = rank * kThreads + glist[gi] * kPer + sub + it * step;
+        if (v < nv) {
+          float f[VEC];
+          unpack(vec_at(v), f);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) offer(f[j], head + v * VEC + j);
+        }
+      }
+      if (has_head) offer(to_f<T>(x[tid]), tid);
+      if (has_tail) offer(to_f<T>(x[tail0 + tid]), tail0 + tid);
+    };
+    auto rank_candidates = [&]() {
+      const int n = ncand;
+      for (int i = tid; i < n; i += kThreads) {
+        const uint64_t k = cand[i];
+        int r = 0;
+        for (int j = 0; j < n; ++j) r += cand[j] > k;
+        if (r < top) list[r] = k;
+      }
+    };
+    bool search = !(t.l == t.l);  // NaN in the CTA's share (its values are not in the groups' largest)
+    if (!search) {
+      collect(false);
+      __syncthreads();
+      if (ncand <= kCand) {
+        rank_candidates();
+      } else {
+        __syncthreads();  // every thread has read ncand
+        if (tid == 0) ncand = 0;
+        __syncthreads();
+        collect(true);
+        __syncthreads();
+        search = ncand > kCand;
+        if (!search) {
+          rank_candidates();
+          // equal ones, in the order of their indices
+          int have = ncand;
+          auto equal = [&](int c, uint32_t i0, uint32_t mask) {  // c of them here, at i0 + the bits of mask
+            int inc = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const int y = __shfl_up_sync(0xffffffffu, inc, o);
+              if (lane >= o) inc += y;
+            }
+            if (lane == 31) wcount[warp] = inc;
+            __syncthreads();
+            int before = 0, total = 0;
+            for (int w = 0; w < kWarps; ++w) {
+              if (w < warp) before += wcount[w];
+              total += wcount[w];
+            }
+            int at = have + before + inc - c;
+            while (mask && at < top) {
+              list[at++] = make_key(tau, i0 + __ffs(mask) - 1);
+              mask &= mask - 1;
+            }
+            have += total;
+            __syncthreads();
+          };
+          {
+            const bool e = has_head && to_f<T>(x[tid]) == tau;
+            equal(e, tid, e);
+          }
+          for (int v = rank * kThreads; v < nv && have < top; v += step) {
+            uint32_t mask = 0;
+            if (v + tid < nv) {
+              float f[VEC];
+              unpack(vec_at(v + tid), f);
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) mask |= (f[j] == tau ? 1u : 0u) << j;
+            }
+            equal(__popc(mask), (uint32_t)(head + (v + tid) * VEC), mask);
+          }
+          if (have < top) {
+            const bool e = has_tail && to_f<T>(x[tail0 + tid]) == tau;
+            equal(e, tail0 + tid, e);
+          }
+        }
+      }
+    }
+    if (search) {  // the largest key below the last one found, `top` times
+      uint64_t last = ~0ull;
+      for (int k = 0; k < top; ++k) {
+        uint64_t mine = 0;
+        auto offer = [&](float f, int i) {
+          const uint64_t key = make_key(f, (uint32_t)i);
+          if (key < last && key > mine) mine = key;
+        };
+        for (int v = v0; v < nv; v += step) {
+          float f[VEC];
+          unpack(vec_at(v), f);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) offer(f[j], head + v * VEC + j);
+        }
+        if (has_head) offer(to_f<T>(x[tid]), tid);
+        if (has_tail) offer(to_f<T>(x[tail0 + tid]), tail0 + tid);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint64_t y = __shfl_xor_sync(0xffffffffu, mine, o);
+          mine = y > mine ? y : mine;
+        }
+        if (lane == 0) wkey[warp] = mine;
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w) mine = wkey[w] > mine ? wkey[w] : mine;
+        if (tid == 0) list[k] = mine;
+        last = mine;
+        __syncthreads();
+        if (last == 0) break;  // the CTA's share has no more
+      }
+    }
+    __syncthreads();
+  }
+
+  // ---- the CTAs of a row meet in the first ----
+  if (C > 1) {
+    if (tid < top) st_cluster_u64(map_to_rank(&lists[rank][tid], 0), list[tid]);
+    if (tid == 0) st_cluster_f4(map_to_rank(&all[rank], 0), t.m, t.l, t.e, 0.f);
+    cluster_sync();
+    if (rank != 0) return;
+    t = Sums{all[0].x, all[0].y, all[0].z};
+    for (int c = 1; c < C; ++c) t = join(t, Sums{all[c].x, all[c].y, all[c].z});
+    for (int i = tid; i < C * top; i += kThreads) {
+      const uint64_t k = lists[i / top][i % top];
+      if (k == 0) continue;
+      // keys are distinct and each list is in order: its own rank is the place
+      // in its list plus what is larger in the others
+      int r = i % top;
+      for (int c = 0; c < C && r < top; ++c) {
+        if (c == i / top) continue;
+        for (int j = 0; j < top && lists[c][j] > k; ++j) ++r;
+      }
+      if (r < top) list[r] = k;
+    }
+    __syncthreads();
+  }
+
+  const float log_l = logf(t.l);
+  const float m = t.m == -INFINITY ? __int_as_float(0x7fc00000) : t.m;  // nothing but -infinity: no distribution
+  auto logprob = [&](float f) { return (f - m) - log_l; };
+  if (tid == 0) {
+    const int64_t tok = a.tokens[row];
+    a.logprob[row] = tok >= 0 && tok < V ? logprob(to_f<T>(x[tok])) : __int_as_float(0x7fc00000);
+    a.entropy[row] = t.m == -INFINITY ? m : log_l - t.e / t.l;
+  }
+  if (tid < top) {
+    const uint64_t k = list[tid];
+    a.top_ids[row * top + tid] = (int64_t)(~(uint32_t)k);
+    a.top_logprobs[row * top + tid] = logprob(key_value(k));
+  }
+}
+
+// CTAs per row: as many as keep about four to an SM busy, up to 16 (a cluster),
+// while each has at least one 16-byte load for every thread.
+int cluster_of(const LogprobsArgs& a, int vec) {
+  const int64_t want = 4 * (int64_t)num_sms(current_device());
+  int c = 1;
+  while (c < kMaxCluster && a.M * (2 * c) <= want && (int64_t)a.V >= (int64_t)2 * c * kThreads * vec) c *= 2;
+  return c;
+}
+
+template <typename T>
+int launch(const LogprobsArgs& a, cudaStream_t st) {
+  auto kern = logprobs_kernel<T>;
+  const int dev = current_device();
+  static bool configured[64] = {false};
+  if (dev < 0 || dev >= 64) return B200MM_ERR_DEVICE;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return B200MM_ERR_LAUNCH;
+    configured[dev] = true;
+  }
+  const int c = cluster_of(a, 16 / (int)sizeof(T));
+  const dim3 grid((unsigned)(a.M * c));
+  const cudaError_t e = c > 1 ? launch_pdl_cluster(kern, grid, dim3(kThreads), 0, st, c, a, c)
+                              : launch_pdl(kern, grid, dim3(kThreads), 0, st, a, c);
+  return e == cudaSuccess ? B200MM_OK : B200MM_ERR_LAUNCH;
+}
+
+}  // namespace
+
+int logprobs_launch(const LogprobsArgs& a, int dtype, cudaStream_t st) {
+  if (dtype == B200MM_BF16) return launch<__nv_bfloat16>(a, st);
+  if (dtype == B200MM_F16) return launch<__half>(a, st);
+  return launch<float>(a, st);
+}
+
+}  // namespace b200mm

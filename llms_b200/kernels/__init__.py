@@ -10,6 +10,7 @@ from .fused_ffn import TritonFFN, triton_fused_gate_up_silu
 from .fused_qkv import TritonAttention, triton_fused_qkv
 from .kv8 import Int8KV, Int8KVCache, int8_kv_append, int8_kv_decode_attn, int8_kv_expand, int8_kv_step
 from .linear import B200Linear, Int8Linear, b200_linear, int8_linear
+from .logprobs import TokenLogprobs, b200_token_logprobs
 from .quant import (
     Int8Attention,
     Int8FFN,
@@ -27,6 +28,8 @@ __all__ = [
     "int8_kv_decode_attn",
     "int8_kv_expand",
     "int8_kv_step",
+    "TokenLogprobs",
+    "b200_token_logprobs",
     "apply_decode_attn",
     "b200_decode_attn",
     "B200Linear",
