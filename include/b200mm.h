@@ -135,6 +135,34 @@ int b200mm_qkv_w8(const void* x, int64_t ldx,
                   int dtype, void* stream);
 
 /*
+ * 4-bit weights with group scales (no reference counterpart):
+ *   W[n, k] = (u[n, k] - 8) * s[n, k / group], group = 32, 64 or 128,
+ *   w : uint8 [N, K / 2], row stride ldw bytes: u of column 2 i in the low, of
+ *       2 i + 1 in the high half of byte i; 16-byte aligned (address and stride)
+ *   s : `dtype` [N, K / group], row stride lds
+ *   x, y : `dtype` (F16 or BF16); x 16-byte aligned (address and row stride)
+ * K is a multiple of group and at most 65536, N at most 2^24.  y = x W^T, fp32 accumulation, no product rounded;
+ * the gate/up variant y = silu(x Wg^T) * (x Wu^T).  From M = 192 on the
+ * weights are first expanded to `dtype` (rounded once) into the workspace:
+ * b200mm_w4_workspace_size bytes (0 below that), 256-byte aligned, owned by
+ * the stream until the call completes.
+ */
+size_t b200mm_w4_workspace_size(int64_t M, int64_t N, int64_t K, int gate);
+
+int b200mm_linear_w4(const void* x, int64_t ldx,
+                     const uint8_t* w, int64_t ldw, const void* s, int64_t lds, int64_t group,
+                     void* y, int64_t ldy,
+                     int64_t M, int64_t N, int64_t K,
+                     int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+int b200mm_gate_up_silu_w4(const void* x, int64_t ldx,
+                           const uint8_t* wg, const uint8_t* wu, int64_t ldw,
+                           const void* sg, const void* su, int64_t lds, int64_t group,
+                           void* y, int64_t ldy,
+                           int64_t M, int64_t N, int64_t K,
+                           int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Plain bias-free projection, y[m, n] = sum_k x[m,k] * w[n,k], on the same
  * kernel families as b200mm_qkv (decode GEMV, small-batch tensor-core GEMV,
  * tcgen05 GEMM).  Replaces the attention output projection `self.o(attn)`

@@ -110,6 +110,17 @@ SIGNATURES: dict[str, tuple] = {
         ctypes.c_int,
         [_c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p],
     ),
+    "b200mm_w4_workspace_size": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, ctypes.c_int]),
+    "b200mm_linear_w4": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int,
+         _c_p, ctypes.c_size_t, _c_p],
+    ),
+    "b200mm_gate_up_silu_w4": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64,
+         ctypes.c_int, _c_p, ctypes.c_size_t, _c_p],
+    ),
     "b200mm_gqa_decode_workspace_size": (ctypes.c_size_t, [_c_i64] * 5),
     "b200mm_gqa_decode": (
         ctypes.c_int,

@@ -10,6 +10,7 @@
 #include "kv8.cuh"
 #include "logprobs.cuh"
 #include "mla.cuh"
+#include "w4.cuh"
 
 namespace b200mm {
 
@@ -213,6 +214,51 @@ int b200mm_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, void* 
 int b200mm_linear_w8(const void* x, int64_t ldx, const int8_t* w, const float* s, int64_t ldw,
                      void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
   return b200mm_qkv_w8(x, ldx, w, s, ldw, y, ldy, M, N, K, dtype, stream);
+}
+
+namespace {
+int run_w4(W4Args& a, int64_t M, int64_t N, int64_t K, int64_t group, size_t ws_bytes) {
+  if (a.dtype != B200MM_F16 && a.dtype != B200MM_BF16) return B200MM_ERR_DTYPE;
+  if (!fits_i32(M) || !fits_i32(N) || !fits_i32(K) || N < 1 || K < 1) return B200MM_ERR_SHAPE;
+  if (N > (int64_t(1) << 24) || K > 65536) return B200MM_ERR_SHAPE;
+  if ((group != 32 && group != 64 && group != 128) || K % group) return B200MM_ERR_SHAPE;
+  if (a.ldx < K || a.ldw < K / 2 || a.lds < K / group || a.ldy < N) return B200MM_ERR_SHAPE;
+  a.M = (int)M; a.N = (int)N; a.K = (int)K; a.G = (int)group;
+  if (M == 0) return B200MM_OK;
+  if (!a.x || !a.w0 || !a.s0 || !a.y || (a.gate && (!a.w1 || !a.s1))) return B200MM_ERR_ARG;
+  auto al = [](const void* p) { return ((uintptr_t)p & 15u) == 0; };
+  if (!al(a.x) || (a.ldx * 2) % 16 || !al(a.w0) || (a.gate && !al(a.w1)) || a.ldw % 16) return B200MM_ERR_ALIGN;
+  const size_t need = w4_workspace_bytes(M, N, K, a.gate);
+  if (need > 0 && (!a.ws || ws_bytes < need || ((uintptr_t)a.ws & 255u))) return B200MM_ERR_WORKSPACE;
+  int st = check_device();
+  if (st != B200MM_OK) return st;
+  st = w4_run(a);
+  return st != B200MM_OK ? st : launch_status();
+}
+}  // namespace
+
+size_t b200mm_w4_workspace_size(int64_t M, int64_t N, int64_t K, int gate) {
+  if (M < 0 || N < 1 || K < 1 || N > (int64_t(1) << 24) || K > 65536) return 0;
+  return w4_workspace_bytes(M, N, K, gate != 0);
+}
+
+int b200mm_linear_w4(const void* x, int64_t ldx, const uint8_t* w, int64_t ldw, const void* s, int64_t lds,
+                     int64_t group, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  W4Args a{};
+  a.x = x; a.ldx = ldx; a.w0 = w; a.ldw = ldw; a.s0 = s; a.lds = lds; a.y = y; a.ldy = ldy;
+  a.dtype = dtype; a.ws = workspace; a.stream = static_cast<cudaStream_t>(stream);
+  return run_w4(a, M, N, K, group, workspace_bytes);
+}
+
+int b200mm_gate_up_silu_w4(const void* x, int64_t ldx, const uint8_t* wg, const uint8_t* wu, int64_t ldw,
+                           const void* sg, const void* su, int64_t lds, int64_t group, void* y, int64_t ldy,
+                           int64_t M, int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  W4Args a{};
+  a.x = x; a.ldx = ldx; a.w0 = wg; a.w1 = wu; a.ldw = ldw; a.s0 = sg; a.s1 = su; a.lds = lds; a.y = y; a.ldy = ldy;
+  a.dtype = dtype; a.gate = true; a.ws = workspace; a.stream = static_cast<cudaStream_t>(stream);
+  return run_w4(a, M, N, K, group, workspace_bytes);
 }
 
 int b200mm_linear_peer(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K,

@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsArgs a
   const int64_t row = blockIdx.x / C;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const int V = a.V, top = a.top;
+  if (C > 1) cluster_arrive();
   pdl_trigger();
   pdl_wait();
 
@@ -343,6 +344,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsArgs a
 
   // ---- the CTAs of a row meet in the first ----
   if (C > 1) {
+    cluster_wait();
     if (tid < top) st_cluster_u64(map_to_rank(&lists[rank][tid], 0), list[tid]);
     if (tid == 0) st_cluster_f4(map_to_rank(&all[rank], 0), t.m, t.l, t.e, 0.f);
     cluster_sync();

@@ -1,0 +1,423 @@
+// Projections with 4-bit weights and group scales:
+//   y[m, n] = epilogue(sum_k x[m, k] (u[n, k] - 8) s[n, k / G]),  G = 32, 64 or 128.
+//
+// Up to 64 rows of x the call is a stream of the weights (0.5 byte each), at
+// 13e12 weights a second on this GPU: one fp32 multiply-add per weight on the
+// CUDA cores would already take longer than the stream, so the products run on
+// mma.sync m16n8k16 from one row of x on, and what is left per weight is its
+// way from four bits to sixteen:
+//   * a warp owns 16 weight rows; lane l reads 16 bytes (32 weights) of rows
+//     l / 4 and l / 4 + 8 as they lie in memory, a chunk of 128 columns per warp;
+//   * the products of one instruction have to lie in one group, so for G = 64
+//     and 32 the four lanes of a row exchange words (one round of shuffles, or
+//     two: a 4 x 4 transpose).  The order of k inside a group is free: x is
+//     staged in shared memory in the order that the lanes hold the weights;
+//   * four bits under the exponent of 2^7 (bf16; 2^10 for fp16) are 128 + u:
+//     one logic instruction per pair, one packed subtraction, exact.  Pairs are
+//     the weights 4 apart in a 32-bit word;
+//   * a group's products are summed in fp32 in accumulators of their own, which
+//     its scale then joins to the row's: no product is rounded;
+//   * K is split over a cluster of CTAs with 128 weight rows each, and the
+//     partial sums meet in distributed shared memory: no workspace, no atomics;
+//   * before griddepcontrol.wait a CTA only asks for its first weights in L2.
+// More rows run in chunks of 64, or, from kDenseRows on, the weights
+// are expanded to 16 bits (rounded once: the tcgen05 GEMM's operands are
+// 16-bit) into the caller's workspace and the dense GEMM takes them.
+#include "w4.cuh"
+
+#include <type_traits>
+
+#include "dense.cuh"
+
+namespace b200mm {
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kRows = 16 * kWarps;  // weight rows per CTA (and matrix)
+constexpr int kChunk = 128;         // columns per warp and step
+constexpr int kMaxRows = 64;        // rows of x per launch
+constexpr int kDenseRows = 192;     // from here on: expand and run the dense GEMM
+constexpr size_t kFenceBytes = 16;  // of workspace that the memset between the two writes
+
+struct W4Params {
+  const void* x; int64_t ldx;
+  const uint8_t* w[2]; int64_t ldw;
+  const void* s[2]; int64_t lds;
+  void* y; int64_t ldy;
+  int M, N, K;
+  int kslice;  // columns per cluster rank (multiple of kChunk)
+};
+
+template <typename T> struct Nib;
+template <> struct Nib<__nv_bfloat16> {
+  // weights i and i + 4 of a word -> (u - 8) pair
+  __device__ __forceinline__ static uint32_t pair(uint32_t w, int i) {
+    const uint32_t h = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&h), __float2bfloat162_rn(136.f));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ __forceinline__ static void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Nib<__half> {
+  __device__ __forceinline__ static uint32_t pair(uint32_t w, int i) {
+    const uint32_t h = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __float2half2_rn(1032.f));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ __forceinline__ static void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+// First column (inside a chunk) of the 8 weights that lane c of a row holds in
+// word j after spread(): words j of the four lanes lie in one group.
+template <int G>
+__device__ __forceinline__ int word_col(int j, int c) {
+  if (G == 128) return 32 * c + 8 * j;
+  if (G == 64) return 64 * (j >> 1) + 32 * (c & 1) + 16 * (c >> 1) + 8 * (j & 1);
+  return 32 * j + 8 * c;
+}
+template <int G>
+__device__ __forceinline__ void spread(uint32_t (&w)[4], int c) {
+  if constexpr (G <= 64) {  // the far half of the words with the lane two away
+    const bool up = c & 2;
+    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, up ? w[0] : w[2], 2);
+    const uint32_t r1 = __shfl_xor_sync(0xffffffffu, up ? w[1] : w[3], 2);
+    if (up) {
+      w[0] = r0;
+      w[1] = r1;
+    } else {
+      w[2] = r0;
+      w[3] = r1;
+    }
+  }
+  if constexpr (G == 32) {  // and every other word with the neighbour
+    const bool up = c & 1;
+    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, up ? w[0] : w[1], 1);
+    const uint32_t r1 = __shfl_xor_sync(0xffffffffu, up ? w[2] : w[3], 1);
+    if (up) {
+      w[0] = r0;
+      w[2] = r1;
+    } else {
+      w[1] = r0;
+      w[3] = r1;
+    }
+  }
+}
+
+// MT: n-tiles of 8 rows of x; CS: CTAs of a cluster (K split).
+template <typename T, int MT, int G, bool GATE, int CS>
+__global__ void __launch_bounds__(kThreads) w4_kernel(const __grid_constant__ W4Params p) {
+  constexpr int NM = GATE ? 2 : 1;
+  constexpr int MP = 8 * MT;
+  constexpr int U = GATE ? 2 : 4;      // chunks in flight per warp
+  constexpr int GPC = kChunk / G;      // groups per chunk
+  constexpr int WPG = 4 / GPC;         // words of a lane per group
+  constexpr int RPO = kRows / CS;      // rows finished per CTA of the cluster
+  constexpr int RP = MP + 2;           // pitch of the partial sums (even: float2 stores)
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const int xpitch = p.kslice + 32;    // elements: rows of x 64 bytes apart in the banks
+  T* xs = reinterpret_cast<T*>(smem_raw);                                             // [MP][xpitch]
+  float* red = reinterpret_cast<float*>(smem_raw + (size_t)MP * xpitch * sizeof(T));  // [NM][CS][RPO][RP]
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = lane >> 2, c = lane & 3;
+  const uint32_t rank = cluster_rank();
+  const int group = blockIdx.x / CS;
+  const int row_lo = group * kRows + 16 * warp + r, row_hi = row_lo + 8;
+  const bool v_lo = row_lo < p.N, v_hi = row_hi < p.N;
+  const int k_begin = (int)rank * p.kslice;
+  const int k_end = min(p.K, k_begin + p.kslice);
+  const int nchunks = k_end > k_begin ? (k_end - k_begin + kChunk - 1) / kChunk : 0;
+
+  cluster_arrive();
+  // the CTA's weights on their way to L2 (nothing is read before the wait)
+  for (int mtx = 0; mtx < NM; ++mtx) {
+    const int lines = (max(k_end - k_begin, 0) / 2 + 127) / 128;
+    for (int i = threadIdx.x; i < kRows * lines; i += kThreads) {
+      const int row = group * kRows + i / lines;
+      if (row < p.N) prefetch_l2(p.w[mtx] + (int64_t)row * p.ldw + k_begin / 2 + (i % lines) * 128);
+    }
+  }
+  pdl_trigger();
+  pdl_wait();
+
+  const uint8_t* wp[NM][2];
+  const T* sp[NM][2];
+#pragma unroll
+  for (int mtx = 0; mtx < NM; ++mtx) {
+    wp[mtx][0] = p.w[mtx] + (int64_t)(v_lo ? row_lo : 0) * p.ldw + k_begin / 2 + 16 * c;
+    wp[mtx][1] = p.w[mtx] + (int64_t)(v_hi ? row_hi : 0) * p.ldw + k_begin / 2 + 16 * c;
+    const T* s = static_cast<const T*>(p.s[mtx]);
+    sp[mtx][0] = s + (int64_t)(v_lo ? row_lo : 0) * p.lds + k_begin / G + c * GPC / 4;
+    sp[mtx][1] = s + (int64_t)(v_hi ? row_hi : 0) * p.lds + k_begin / G + c * GPC / 4;
+  }
+  uint4 wv[U][NM][2];
+  float sv[U][NM][2];  // of this lane's group of the chunk
+  auto load = [&](int u, int ch) {
+    const bool in = ch < nchunks && k_begin + ch * kChunk + 32 * c < k_end;
+#pragma unroll
+    for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool ok = in && (h ? v_hi : v_lo);
+        wv[u][mtx][h] = ok ? __ldcs(reinterpret_cast<const uint4*>(wp[mtx][h] + (int64_t)ch * (kChunk / 2)))
+                           : make_uint4(0, 0, 0, 0);
+        sv[u][mtx][h] = ok ? to_f<T>(sp[mtx][h][(int64_t)ch * GPC]) : 0.f;
+      }
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) load(u, u);
+
+  // stage x[:, k_begin : k_end) (zero past M and k_end): 8 columns from
+  // word_col(j, c) lie at 16-byte place 4 j + c of their chunk, in the order of the
+  // pairs 0 4 1 5 2 6 3 7
+  {
+    const T* x = static_cast<const T*>(p.x);
+    const int words = nchunks * (kChunk / 8);
+    for (int i = threadIdx.x; i < MP * words; i += kThreads) {
+      const int m = i / words, wd = i - m * words;
+      const int place = wd % 16, ch = wd / 16;
+      const int k = k_begin + ch * kChunk + word_col<G>(place / 4, place % 4);
+      uint32_t o[4] = {0, 0, 0, 0};
+      if (m < p.M && k < k_end) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k);
+        o[0] = __byte_perm(v.x, v.z, 0x5410);
+        o[1] = __byte_perm(v.x, v.z, 0x7632);
+        o[2] = __byte_perm(v.y, v.w, 0x5410);
+        o[3] = __byte_perm(v.y, v.w, 0x7632);
+      }
+      *reinterpret_cast<uint4*>(xs + (int64_t)m * xpitch + ch * kChunk + place * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+  __syncthreads();
+
+  float acc[NM][MT][4];
+#pragma unroll
+  for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[mtx][t][e] = 0.f;
+
+  const T* xl = xs + (int64_t)r * xpitch + 8 * c;
+  for (int c0 = 0; c0 < nchunks; c0 += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int ch = c0 + u;
+      if (ch >= nchunks) break;
+#pragma unroll
+      for (int mtx = 0; mtx < NM; ++mtx) {
+        uint32_t lo[4] = {wv[u][mtx][0].x, wv[u][mtx][0].y, wv[u][mtx][0].z, wv[u][mtx][0].w};
+        uint32_t hi[4] = {wv[u][mtx][1].x, wv[u][mtx][1].y, wv[u][mtx][1].z, wv[u][mtx][1].w};
+        spread<G>(lo, c);
+        spread<G>(hi, c);
+#pragma unroll
+        for (int g = 0; g < GPC; ++g) {
+          float part[MT][4];
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[t][e] = 0.f;
+#pragma unroll
+          for (int jj = 0; jj < WPG; ++jj) {
+            const int j = g * WPG + jj;
+            uint32_t a[2][4];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              a[q][0] = Nib<T>::pair(lo[j], 2 * q);
+              a[q][1] = Nib<T>::pair(hi[j], 2 * q);
+              a[q][2] = Nib<T>::pair(lo[j], 2 * q + 1);
+              a[q][3] = Nib<T>::pair(hi[j], 2 * q + 1);
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              const uint4 b = *reinterpret_cast<const uint4*>(xl + (int64_t)(8 * t) * xpitch + ch * kChunk + 32 * j);
+              Nib<T>::mma(part[t], a[0], b.x, b.y);
+              Nib<T>::mma(part[t], a[1], b.z, b.w);
+            }
+          }
+          // lane quad + (4 / GPC) g holds the group's scales
+          const float s_lo = GPC == 1 ? sv[u][mtx][0] : __shfl_sync(0xffffffffu, sv[u][mtx][0], (lane & 28) + g * (4 / GPC));
+          const float s_hi = GPC == 1 ? sv[u][mtx][1] : __shfl_sync(0xffffffffu, sv[u][mtx][1], (lane & 28) + g * (4 / GPC));
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            acc[mtx][t][0] = fmaf(part[t][0], s_lo, acc[mtx][t][0]);
+            acc[mtx][t][1] = fmaf(part[t][1], s_lo, acc[mtx][t][1]);
+            acc[mtx][t][2] = fmaf(part[t][2], s_hi, acc[mtx][t][2]);
+            acc[mtx][t][3] = fmaf(part[t][3], s_hi, acc[mtx][t][3]);
+          }
+        }
+      }
+      load(u, ch + U);
+    }
+  }
+
+  // partial sums to the CTA that finishes their rows
+  cluster_wait();
+  {
+    const int owner = (16 * warp) / RPO;
+    const int lrow = (16 * warp) % RPO + r;
+#pragma unroll
+    for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          float* dst = red + ((int64_t)(mtx * CS + rank) * RPO + lrow + 8 * hf) * RP + 8 * t + 2 * c;
+          st_cluster_f2(map_to_rank(dst, (uint32_t)owner), acc[mtx][t][2 * hf], acc[mtx][t][2 * hf + 1]);
+        }
+  }
+  cluster_sync();
+  T* y = static_cast<T*>(p.y);
+  for (int i = threadIdx.x; i < RPO * p.M; i += kThreads) {
+    const int m = i / RPO, lr = i % RPO;
+    const int n = group * kRows + RPO * (int)rank + lr;
+    if (n >= p.N) continue;
+    float v[NM];
+#pragma unroll
+    for (int mtx = 0; mtx < NM; ++mtx) {
+      v[mtx] = 0.f;
+#pragma unroll
+      for (int q = 0; q < CS; ++q) v[mtx] += red[((int64_t)(mtx * CS + q) * RPO + lr) * RP + m];
+    }
+    y[(int64_t)m * p.ldy + n] = from_f<T>(GATE ? silu_mul(v[0], v[NM - 1]) : v[0]);
+  }
+}
+
+// The dense GEMM reads weights before griddepcontrol.wait, and these are fresh:
+// no early trigger here, and a full dependency (a memset) between the two.
+// 32 weights of a row per thread: 16-bit weights (q s, rounded once), row-major [N, K].
+template <typename T>
+__global__ void __launch_bounds__(256) w4_expand_kernel(const uint8_t* w, int64_t ldw, const T* s, int64_t lds, T* out,
+                                                        int N, int K, int G) {
+  pdl_wait();
+  const int per = K / 32;
+  const int64_t n = (int64_t)N * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per;
+    const int k = (int)(i - row * per) * 32;
+    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(w + row * ldw + k / 2));
+    const float sc = to_f<T>(s[row * lds + k / G]);
+    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+    T* dst = out + row * K + k;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      T o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = from_f<T>((float)((int)((words[j] >> (4 * e)) & 15u) - 8) * sc);
+      *reinterpret_cast<uint4*>(dst + 8 * j) = *reinterpret_cast<const uint4*>(o);
+    }
+  }
+}
+
+size_t smem_bytes(int MT, bool gate, int kslice) {
+  const int MP = 8 * MT;
+  return (size_t)MP * (kslice + 32) * 2 + (size_t)(gate ? 2 : 1) * kRows * (MP + 2) * sizeof(float);
+}
+constexpr size_t kMaxSmem = 220 * 1024;
+
+int kslice_of(int K, int cs) {
+  const int per = (K + cs - 1) / cs;
+  return (per + kChunk - 1) / kChunk * kChunk;
+}
+
+template <typename T, int MT, int G, bool GATE, int CS>
+int launch_w4(const W4Params& p, cudaStream_t st) {
+  auto kern = w4_kernel<T, MT, G, GATE, CS>;
+  const size_t smem = smem_bytes(MT, GATE, p.kslice);
+  if (smem > kMaxSmem) return B200MM_ERR_SHAPE;
+  static int configured[64] = {0};
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return B200MM_ERR_DEVICE;
+  if ((int)smem > configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem) != cudaSuccess)
+      return B200MM_ERR_LAUNCH;
+    configured[dev] = (int)kMaxSmem;
+  }
+  const int groups = (p.N + kRows - 1) / kRows;
+  return launch_pdl_cluster(kern, dim3(groups * CS), dim3(kThreads), smem, st, CS, p) == cudaSuccess ? B200MM_OK
+                                                                                                  : B200MM_ERR_LAUNCH;
+}
+
+template <typename T, int MT, int G>
+int launch_gate(const W4Params& p, bool gate, cudaStream_t st) {
+  return gate ? launch_w4<T, MT, G, true, 8>(p, st) : launch_w4<T, MT, G, false, 8>(p, st);
+}
+template <typename T, int MT>
+int launch_group(const W4Params& p, int G, bool gate, cudaStream_t st) {
+  if (G == 128) return launch_gate<T, MT, 128>(p, gate, st);
+  if (G == 64) return launch_gate<T, MT, 64>(p, gate, st);
+  return launch_gate<T, MT, 32>(p, gate, st);
+}
+template <typename T>
+int launch_rows(const W4Params& p, int G, bool gate, cudaStream_t st) {
+  if (p.M <= 8) return launch_group<T, 1>(p, G, gate, st);
+  if (p.M <= 16) return launch_group<T, 2>(p, G, gate, st);
+  if (p.M <= 32) return launch_group<T, 4>(p, G, gate, st);
+  return launch_group<T, 8>(p, G, gate, st);
+}
+
+// Rows of x per launch: as many (a power of two from 8, at most 64) as leave room for the K slice in shared memory.
+int rows_per_launch(const W4Args& a) {
+  int m = kMaxRows;
+  while (m > 8 && smem_bytes(m / 8, a.gate, kslice_of(a.K, 8)) > kMaxSmem) m /= 2;
+  return m;
+}
+
+template <typename T>
+int run_t(const W4Args& a) {
+  if (a.M >= kDenseRows) {
+    T* dense[3];
+    for (int i = 0; i < 3; ++i) dense[i] = static_cast<T*>(a.ws) + i * (int64_t)a.N * a.K;
+    for (int i = 0; i < (a.gate ? 2 : 1); ++i) {
+      const int64_t want = ((int64_t)a.N * (a.K / 32) + 255) / 256;
+      const unsigned grid = (unsigned)(want < 16384 ? want : 16384);
+      if (launch_pdl(w4_expand_kernel<T>, dim3(grid), dim3(256), 0, a.stream, i ? a.w1 : a.w0, a.ldw,
+                     static_cast<const T*>(i ? a.s1 : a.s0), a.lds, dense[i], a.N, a.K, a.G) != cudaSuccess)
+        return B200MM_ERR_LAUNCH;
+    }
+    if (cudaMemsetAsync(dense[a.gate ? 2 : 1], 0, kFenceBytes, a.stream) != cudaSuccess) return B200MM_ERR_LAUNCH;
+    DenseArgs d{};
+    d.x = a.x; d.ldx = a.ldx; d.w0 = dense[0]; d.ldw0 = a.K;
+    if (a.gate) { d.w1 = dense[1]; d.ldw1 = a.K; }
+    d.y = a.y; d.ldy = a.ldy; d.M = a.M; d.N = a.N; d.K = a.K;
+    d.dtype = a.dtype; d.gate = a.gate; d.stream = a.stream;
+    return dense_dispatch(d);
+  }
+  const int step = rows_per_launch(a);
+  for (int m0 = 0; m0 < a.M; m0 += step) {
+    W4Params p{};
+    p.x = static_cast<const T*>(a.x) + (int64_t)m0 * a.ldx; p.ldx = a.ldx;
+    p.w[0] = a.w0; p.w[1] = a.w1; p.ldw = a.ldw;
+    p.s[0] = a.s0; p.s[1] = a.s1; p.lds = a.lds;
+    p.y = static_cast<T*>(a.y) + (int64_t)m0 * a.ldy; p.ldy = a.ldy;
+    p.M = a.M - m0 < step ? a.M - m0 : step; p.N = a.N; p.K = a.K;
+    p.kslice = kslice_of(a.K, 8);
+    const int st = launch_rows<T>(p, a.G, a.gate, a.stream);
+    if (st != B200MM_OK) return st;
+  }
+  return B200MM_OK;
+}
+
+}  // namespace
+
+size_t w4_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gate) {
+  return M >= kDenseRows ? (size_t)(gate ? 2 : 1) * N * K * 2 + kFenceBytes : 0;
+}
+
+int w4_run(const W4Args& a) {
+  return a.dtype == B200MM_BF16 ? run_t<__nv_bfloat16>(a) : run_t<__half>(a);
+}
+
+}  // namespace b200mm

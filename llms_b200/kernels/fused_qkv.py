@@ -16,6 +16,7 @@ from torch import nn
 from .. import _capi
 from ._eager import RMSNorm, rope
 from .glue import fits_qk_norm_rope, qk_norm_rope_cache
+from .kv8 import Int8KVCache
 
 
 def _check_qkv_args(x: torch.Tensor, W_qkv: torch.Tensor, n_q: int, n_k: int) -> None:
@@ -86,6 +87,24 @@ def _one_buffer(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tens
     return q.as_strided(q.shape[:-1] + (n_q + 2 * n_k,), q.stride())
 
 
+def new_tokens(attn, qf: torch.Tensor, kf: torch.Tensor, vf: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
+    """q (B, H, T, D), k and v (B, KV, T, D) of new tokens after QK-norm and
+    RoPE, for a cache that stores them itself.  ``qf`` / ``kf`` / ``vf``: the
+    projections (B, T, heads * D); ``cos`` / ``sin``: the tokens' rows of the tables."""
+    B, T = qf.shape[:2]
+    H, KV, D = attn.num_heads, attn.num_kv_heads, attn.head_dim
+    flat = _one_buffer(qf, kf, vf)
+    if T == 1 and flat is not None and fits_qk_norm_rope(flat, attn.q_norm, attn.k_norm, cos, D):
+        k, v = torch.empty(2, B, KV, 1, D, dtype=flat.dtype, device=flat.device)
+        q = qk_norm_rope_cache(flat, attn.q_norm, attn.k_norm, cos, sin, num_heads=H, num_kv_heads=KV, head_dim=D,
+                               k_cache=k, v_cache=v, pos=0)
+        return q, k, v
+    q = attn.q_norm(qf.reshape(B, T, H, D)).transpose(1, 2)
+    k = attn.k_norm(kf.reshape(B, T, KV, D)).transpose(1, 2)
+    v = vf.reshape(B, T, KV, D).transpose(1, 2)
+    return rope(q, cos, sin), rope(k, cos, sin), v
+
+
 class TritonAttention(nn.Module):
     """Drop-in for the engine's GQA ``Attention`` whose q/k/v projections run
     as one fused B200 launch against a pre-concatenated ``W_qkv``.
@@ -139,6 +158,10 @@ class TritonAttention(nn.Module):
         qf, kf, vf = self.project_qkv(x)
         end = start_pos + T
         flat = _one_buffer(qf, kf, vf)
+        if isinstance(kv_cache, Int8KVCache):
+            q, k, v = new_tokens(self, qf, kf, vf, cos, sin)
+            attn = kv_cache.attend(q, k, v, layer_idx, start_pos)
+            return self.o(attn.transpose(1, 2).reshape(B, T, self.num_heads * self.head_dim))
         if T == 1 and flat is not None and fits_qk_norm_rope(flat, self.q_norm, self.k_norm, cos, self.head_dim):
             # one launch for q_norm, k_norm, RoPE and the cache write of the
             # decode token (the same rounding as the eager lines below)

@@ -13,6 +13,7 @@ from torch import nn
 
 from .fused_ffn import TritonFFN
 from .fused_qkv import TritonAttention, triton_fused_qkv
+from .int4 import Int4Attention, Int4FFN, Int4Linear, int4_fused_qkv
 from .linear import B200Linear, Int8Linear
 from .quant import Int8Attention, Int8FFN, int8_fused_qkv
 
@@ -21,7 +22,7 @@ def apply_triton_kernels(model: nn.Module, *, fused_ffn: bool = True, fused_qkv:
     """Replace each layer's ``ffn`` with :class:`TritonFFN` and ``attn`` with
     :class:`TritonAttention` (idempotent; returns ``model``)."""
     for block in model.layers:
-        if fused_ffn and not isinstance(block.ffn, (TritonFFN, Int8FFN)):
+        if fused_ffn and not isinstance(block.ffn, (TritonFFN, Int8FFN, Int4FFN)):
             block.ffn = TritonFFN.from_eager(block.ffn)
         if fused_qkv and not isinstance(block.attn, TritonAttention) and hasattr(block.attn, "v"):
             block.attn = TritonAttention.from_eager(block.attn)
@@ -32,12 +33,33 @@ def apply_int8_kernels(model: nn.Module, *, ffn: bool = True, qkv: bool = True) 
     """Quantise each layer's gate/up and q/k/v weights to int8 per output row
     and swap in :class:`Int8FFN` / :class:`Int8Attention` (idempotent)."""
     for block in model.layers:
-        if ffn and not isinstance(block.ffn, Int8FFN):
+        if ffn and not isinstance(block.ffn, (Int8FFN, Int4FFN)):
             block.ffn = Int8FFN.from_eager(block.ffn)
         if qkv and not isinstance(block.attn, Int8Attention) and (
             hasattr(block.attn, "v") or hasattr(block.attn, "W_qkv")
         ):
             block.attn = Int8Attention.from_eager(block.attn)
+    return model
+
+
+def apply_int4_kernels(model: nn.Module, *, group: int = 128, ffn: bool = True, qkv: bool = True, o: bool = True,
+                       down: bool = True, lm_head: bool = False) -> nn.Module:
+    """Quantise each layer's projections to 4 bits with a scale per ``group``
+    columns and swap in :class:`Int4FFN` / :class:`Int4Attention`, with
+    :class:`Int4Linear` for ``attn.o`` / ``ffn.down`` (and, with ``lm_head=True``,
+    the LM head).  Modules that hold 8- or 4-bit weights already stay
+    (idempotent; returns ``model``)."""
+    for block in model.layers:
+        if ffn and not isinstance(block.ffn, (Int8FFN, Int4FFN)):
+            block.ffn = Int4FFN.from_eager(block.ffn, group=group)
+        if qkv and (hasattr(block.attn, "v") or hasattr(block.attn, "W_qkv")):
+            block.attn = Int4Attention.from_eager(block.attn, group=group)
+        if o and isinstance(block.attn.o, (nn.Linear, B200Linear)):
+            block.attn.o = Int4Linear.from_linear(block.attn.o, group=group)
+        if down and isinstance(block.ffn.down, (nn.Linear, B200Linear)):
+            block.ffn.down = Int4Linear.from_linear(block.ffn.down, group=group)
+    if lm_head and isinstance(getattr(model, "lm_head", None), (nn.Linear, B200Linear)):
+        model.lm_head = Int4Linear.from_linear(model.lm_head, group=group)
     return model
 
 
@@ -73,6 +95,10 @@ def prewarm_triton_kernels(model: nn.Module, *, m_values: tuple[int, ...] = (1, 
             ffns.setdefault(("d",) + tuple(m.gate.weight.shape), m)
         elif isinstance(m, Int8FFN):
             ffns.setdefault(("q",) + tuple(m.qg.shape), m)
+        elif isinstance(m, Int4FFN):
+            ffns.setdefault(("4", m.wg.shape[0], 2 * m.wg.shape[1]), m)
+        elif isinstance(m, Int4Attention):
+            attns.setdefault(("4", m.w_qkv.shape[0], 2 * m.w_qkv.shape[1]), m)
         elif isinstance(m, Int8Attention):
             attns.setdefault(("q",) + tuple(m.q_qkv.shape), m)
         elif isinstance(m, TritonAttention):
@@ -84,6 +110,8 @@ def prewarm_triton_kernels(model: nn.Module, *, m_values: tuple[int, ...] = (1, 
             K = key[2]
             if isinstance(ffn, TritonFFN):
                 dev, dt = ffn.gate.weight.device, ffn.gate.weight.dtype
+            elif isinstance(ffn, Int4FFN):
+                dev, dt = ffn.wg.device, ffn.sg.dtype
             else:
                 dev, dt = ffn.qg.device, ffn.down.weight.dtype
             for M in m_values:
@@ -91,7 +119,10 @@ def prewarm_triton_kernels(model: nn.Module, *, m_values: tuple[int, ...] = (1, 
         for key, attn in attns.items():
             K = key[2]
             for M in m_values:
-                if isinstance(attn, Int8Attention):
+                if isinstance(attn, Int4Attention):
+                    x = torch.zeros((1, M, K), dtype=attn.s_qkv.dtype, device=attn.w_qkv.device)
+                    int4_fused_qkv(x, attn.w_qkv, attn.s_qkv, n_q=attn.n_q, n_k=attn.n_k)
+                elif isinstance(attn, Int8Attention):
                     x = torch.zeros((1, M, K), dtype=attn.o.weight.dtype, device=attn.q_qkv.device)
                     int8_fused_qkv(x, attn.q_qkv, attn.s_qkv, n_q=attn.n_q, n_k=attn.n_k)
                 else:

@@ -23,8 +23,10 @@ import torch.nn.functional as F
 from torch import nn
 
 from .kernels._eager import RMSNorm, rope
-from .kernels.fused_qkv import _one_buffer
+from .kernels.fused_qkv import _one_buffer, new_tokens
 from .kernels.glue import fits_qk_norm_rope, fits_rms_norm, qk_norm_rope_cache, rms_norm
+from .kernels.kv8 import Int8KVCache, int8_kv_step
+from .kernels.logprobs import TokenLogprobs, b200_token_logprobs
 from .kernels.quant import Int8Attention, Int8FFN, dequantize_per_row
 
 
@@ -72,6 +74,8 @@ def rope_tables(head_dim: int, max_pos: int, theta: float, device=None):
 def attention_core(q, k, v, kv_cache, layer_idx, start_pos, n_rep, decode_op=None):
     """Cache write + GQA SDPA of engine/attention.py:122-149 (q, k, v: B, H, T, D);
     a single-query step goes to ``decode_op`` when one is set (:138-145)."""
+    if isinstance(kv_cache, Int8KVCache):
+        return kv_cache.attend(q, k, v, layer_idx, start_pos)
     B, _, T, _ = q.shape
     end = start_pos + T
     kv_cache.k[layer_idx][:B, :, start_pos:end] = k
@@ -110,10 +114,16 @@ def static_decode_attention(attn, x, kv_cache, layer_idx, cos, sin, pos, tables=
     capacity (``max_seq_len`` rows, masked) at every position, so a step
     costs time for the capacity, not the current length; and
     ``attn.decode_attn_op`` is not used here (the GQA decode kernel takes the
-    length on the host), so a captured step runs torch's SDPA."""
+    length on the host), so a captured step runs torch's SDPA.  An
+    :class:`Int8KVCache` has neither: its kernels read the position on the
+    device and attend to the tokens that are there."""
     B = x.shape[0]
     H, KV, D = attn.num_heads, attn.num_kv_heads, attn.head_dim
     qf, kf, vf = _project_qkv(attn, x)
+    if isinstance(kv_cache, Int8KVCache):
+        q, k, v = new_tokens(attn, qf, kf, vf, cos, sin)
+        a = int8_kv_step(q, k, v, kv_cache.layers[layer_idx], pos, scale=D ** -0.5)
+        return attn.o(a.transpose(1, 2).reshape(B, 1, H * D))
     kc, vc = kv_cache.k[layer_idx][:B], kv_cache.v[layer_idx][:B]
     flat = _one_buffer(qf, kf, vf)
     if (tables is not None and flat is not None and kc.dtype == flat.dtype
@@ -264,9 +274,24 @@ class Qwen3Model(nn.Module):
             h = h + blk.ffn(blk.norm2(h))
         return self.lm_head(self.final_norm(h))
 
-    def alloc_cache(self, max_seq_len, *, max_batch=1, dtype=None, device=None) -> KVCache:
-        p = self.lm_head.weight
-        return KVCache.alloc(num_layers=len(self.layers), max_batch=max_batch,
+    @torch.inference_mode()
+    def score(self, input_ids: torch.Tensor, kv_cache, *, top: int = 0, start_pos=None) -> TokenLogprobs:
+        """Log probabilities of ``input_ids`` (B, T) under the model, each given
+        the tokens before it: one forward pass, then
+        :func:`b200_token_logprobs` of tokens 1..T-1 (shape (B, T - 1)) with
+        the entropy and the ``top`` alternatives at each place.  The cache
+        holds the T tokens afterwards."""
+        logits = self(input_ids, kv_cache, start_pos)
+        # all rows, so that the logits need no copy; nothing follows the last token
+        following = F.pad(input_ids[:, 1:], (0, 1), value=-1)
+        return TokenLogprobs(*(r[:, :-1] for r in b200_token_logprobs(logits, following, top=top)))
+
+    def alloc_cache(self, max_seq_len, *, max_batch=1, dtype=None, device=None,
+                    int8: bool = False) -> KVCache | Int8KVCache:
+        """An empty cache; ``int8``: held in 8 bits (``dtype`` then is the
+        activations' type)."""
+        p = self.embed.weight
+        return (Int8KVCache if int8 else KVCache).alloc(num_layers=len(self.layers), max_batch=max_batch,
                              num_kv_heads=self.shape.num_key_value_heads, max_seq_len=max_seq_len,
                              head_dim=self.shape.head_dim, dtype=dtype or p.dtype, device=device or p.device)
 
@@ -324,7 +349,7 @@ class GraphedDecodeStep:
     the row the first real step writes anyway."""
 
     def __init__(self, model: Qwen3Model, kv_cache: KVCache, batch: int) -> None:
-        dev = model.lm_head.weight.device
+        dev = model.embed.weight.device
         self.model, self.cache = model, kv_cache
         self.ids = torch.zeros(batch, 1, dtype=torch.long, device=dev)
         self.pos = torch.full((1,), kv_cache.cur_len, dtype=torch.long, device=dev)
@@ -338,11 +363,14 @@ class GraphedDecodeStep:
             self.logits = model.forward_static(self.ids, kv_cache, self.pos)
 
     def __call__(self, ids: torch.Tensor, pos: int) -> torch.Tensor:
-        S = self.cache.k[0].shape[2]
+        int8 = isinstance(self.cache, Int8KVCache)
+        S = self.cache.capacity if int8 else self.cache.k[0].shape[2]
         if not 0 <= pos < S:
             raise ValueError(f"position {pos} is outside the cache (rows 0..{S - 1})")
         if tuple(ids.shape) != tuple(self.ids.shape):
             raise ValueError(f"ids shape {tuple(ids.shape)} != the captured step's {tuple(self.ids.shape)}")
+        if int8:
+            self.cache.seek(pos)
         self.ids.copy_(ids)
         self.pos.fill_(pos)
         self.graph.replay()

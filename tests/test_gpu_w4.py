@@ -1,0 +1,197 @@
+"""Projections with 4-bit weights vs their formula in 64 bits.
+
+No product is rounded below 192 rows.  The sums: K / 16 instructions' sums,
+K / group scaled ones, 8 partial ones, each rounded (or cut) within 2^-23 of what
+stands there, at most mass = sum_k |x w|; then half a step of the output's type.
+From 192 rows on each weight is rounded too, half a step of its type."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    import llms_b200.kernels  # noqa: F401
+
+
+def _weights(N, K, G, dtype, seed=0):
+    """Every 4-bit value, scales of both signs, zero ones, ones far apart."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.randint(0, 256, (N, K // 2), device="cuda", generator=g, dtype=torch.uint8)
+    s = torch.randn(N, K // G, device="cuda", generator=g) * 0.01
+    s[::7, ::2] = 0
+    s[1::5] *= 100
+    return w, s.to(dtype)
+
+
+def _x(M, K, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(100 + seed)
+    return torch.randn(M, K, device="cuda", generator=g).to(dtype)
+
+
+def _dense(w, s):
+    u = torch.stack((w & 15, w >> 4), -1).view(w.shape[0], -1).double() - 8
+    return u * s.double().repeat_interleave(u.shape[1] // s.shape[1], 1)
+
+
+def _product(x, w, s):
+    """(x W^T, its bound) in 64 bits."""
+    W, K = _dense(w, s), x.shape[1]
+    mass = x.double().abs() @ W.abs().T
+    eps = torch.finfo(x.dtype).eps / 2 if x.shape[0] >= 192 else 0.0
+    return x.double() @ W.T, ((K / 16 + s.shape[1] + 8) * 2.0 ** -23 + eps) * mass
+
+
+def _check_linear(y, x, w, s):
+    want, tol = _product(x, w, s)
+    d = (y.double() - want).abs() - tol - torch.finfo(x.dtype).eps / 2 * want.abs()
+    assert y.dtype == x.dtype and d.max() <= 0, d.max().item()
+
+
+def _check_gate(y, x, wg, sg, wu, su):
+    (g, tg), (u, tu) = _product(x, wg, sg), _product(x, wu, su)
+    want = g * torch.sigmoid(g) * u
+    # |silu'| <= 1.1; the exponential, the quotient and the product: 2^-20 of the value
+    tol = 1.1 * tg * (u.abs() + tu) + (g * torch.sigmoid(g)).abs() * tu + (2.0 ** -20 + torch.finfo(x.dtype).eps / 2) * want.abs()
+    # beyond the type's range the rounding gives infinity, below it steps of the smallest number
+    tol = tol + torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+    want = torch.where(want.abs() > torch.finfo(x.dtype).max, want.sign() * torch.inf, want)
+    fin = want.isfinite()
+    assert torch.equal(y.isfinite(), fin)
+    assert ((y.double() - want).abs() - tol)[fin].max() <= 0
+
+
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 128), (1, 6144, 4096), (2, 130, 256), (7, 127, 1152), (8, 128, 1024), (9, 300, 2176),
+                                   (16, 512, 896), (17, 65, 384), (33, 257, 1280), (64, 640, 640), (65, 96, 512), (150, 200, 256),
+                                   (192, 256, 512), (300, 264, 1024)])
+def test_linear(dtype, G, M, N, K):
+    from llms_b200.kernels import int4_linear
+    x, (w, s) = _x(M, K, dtype), _weights(N, K, G, dtype, seed=M)
+    _check_linear(int4_linear(x, w, s), x, w, s)
+
+
+@pytest.mark.parametrize("K,G", [(32, 32), (64, 32), (96, 32), (160, 32), (64, 64), (192, 64), (320, 64), (1056, 32), (1088, 64),
+                                 (65536, 128)])
+@pytest.mark.parametrize("M", [1, 12])
+def test_columns_that_end_inside_a_chunk(K, G, M):
+    from llms_b200.kernels import int4_linear
+    x, (w, s) = _x(M, K, BF), _weights(70, K, G, BF, seed=K)
+    _check_linear(int4_linear(x, w, s), x, w, s)
+
+
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("M,N,K", [(1, 12288, 4096), (1, 3, 128), (5, 129, 384), (16, 320, 1024), (31, 70, 256), (64, 200, 640),
+                                   (100, 128, 256), (200, 136, 512)])
+def test_gate_up(dtype, G, M, N, K):
+    from llms_b200.kernels import int4_fused_gate_up_silu
+    x = _x(M, K, dtype) * 0.1
+    wg, sg = _weights(N, K, G, dtype, seed=M)
+    wu, su = _weights(N, K, G, dtype, seed=M + 1)
+    _check_gate(int4_fused_gate_up_silu(x, wg, sg, wu, su), x, wg, sg, wu, su)
+
+
+@pytest.mark.parametrize("M", [1, 40])
+def test_x_at_the_ends_of_its_range(M):
+    """bf16 activations beyond fp16's range, and an infinity and a NaN in one row only."""
+    from llms_b200.kernels import int4_linear
+    x, (w, s) = _x(M, 512, BF), _weights(64, 512, 64, BF)
+    x[:, ::3] *= 2.0 ** 60
+    x[:, 1::3] *= 2.0 ** -60
+    _check_linear(int4_linear(x, w, s), x, w, s)
+    if M > 1:
+        x[3, 5], x[7, 9] = torch.inf, torch.nan
+        y = int4_linear(x, w, s)
+        rows = torch.ones(M, dtype=torch.bool, device="cuda")
+        rows[[3, 7]] = False
+        _check_linear(y[rows], x[rows], w, s)
+        assert not y[3].isfinite().any() and y[7].isnan().all()
+
+
+def test_strides_views_and_shapes():
+    from llms_b200.kernels import int4_fused_gate_up_silu, int4_fused_qkv, int4_linear
+    K, N = 256, 96
+    w, s = _weights(2 * N, K, 64, BF, seed=2)
+    big = torch.randn(6, K + 8, device="cuda").to(BF)
+    for x in (big[:, :K], big[:, 8:], big[:, 3:K + 3], big[::2, :K], big[:, :K].reshape(2, 3, K), torch.randn(K, 5, device="cuda").to(BF).t()):
+        y = int4_linear(x, w, s)
+        assert y.shape == (*x.shape[:-1], 2 * N)
+        _check_linear(y.reshape(-1, 2 * N), x.reshape(-1, K), w, s)
+    x = big[:, :K]
+    # rows of a stacked weight, every second row, scales of a larger table, an unaligned weight
+    _check_linear(int4_linear(x, w[N:], s[N:]), x, w[N:], s[N:])
+    _check_linear(int4_linear(x, w[::2], s[::2]), x, w[::2], s[::2])
+    t = torch.zeros(2 * N, 7, device="cuda", dtype=BF)
+    t[:, 2:6] = s
+    _check_linear(int4_linear(x, w, t[:, 2:6]), x, w, s)
+    u = torch.zeros(2 * N * K // 2 + 1, dtype=torch.uint8, device="cuda")[1:].view(2 * N, K // 2)
+    u.copy_(w)
+    _check_linear(int4_linear(x, u, s), x, w, s)
+    _check_gate(int4_fused_gate_up_silu(x, w[:N], s[:N], u[N:], t[N:, 2:6]), x, w[:N], s[:N], w[N:], s[N:])
+    q, k, v = int4_fused_qkv(x, w, s, n_q=N, n_k=N // 2)
+    assert torch.equal(torch.cat((q, k, v), -1), int4_linear(x, w, s)) and k.data_ptr() == q.data_ptr() + 2 * N
+
+
+def test_what_lies_behind_the_output_stays():
+    """Rows of y with a stride of their own, through the C entry."""
+    from llms_b200 import _capi
+    M, N, K, G = 5, 100, 384, 128
+    x, (w, s) = _x(M, K, BF), _weights(N, K, G, BF)
+    y = torch.full((M + 1, 128), 7.0, dtype=BF, device="cuda")
+    st = _capi.lib.b200mm_linear_w4(x.data_ptr(), K, w.data_ptr(), K // 2, s.data_ptr(), K // G, G, y.data_ptr(), 128, M, N, K, 2,
+                                    None, 0, _capi.stream_of(x))
+    assert st == 0
+    _check_linear(y[:M, :N], x, w, s)
+    assert (y[:, N:] == 7).all() and (y[M] == 7).all()
+
+
+@pytest.mark.parametrize("M", [1, 200])
+def test_graphs_streams_and_weights_made_just_before(M):
+    from llms_b200.kernels import dequantize_grouped, int4_linear, quantize_grouped
+    W = (torch.randn(512, 1024, device="cuda") * 0.02).to(BF)
+    x = _x(M, 1024, BF)
+    for _ in range(3):  # weights and x of the same stream, no wait between
+        w, s = quantize_grouped(W, 128)
+        y = int4_linear(x, w, s)
+        assert torch.equal(y, int4_linear(x, w, s))
+        _check_linear(y, x, w, s)
+        W = W.flip(0).contiguous()
+    assert (dequantize_grouped(w, s).double() - _dense(w, s)).abs().max() == 0
+    graphs = []
+    for i in range(2):
+        xi = x.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            yi = int4_linear(int4_linear(xi, w, s)[:, :512].repeat(1, 2), w, s)
+        graphs.append((g, xi, yi, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for r in range(4):
+        for i, (g, xi, yi, st) in enumerate(graphs):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                xi.copy_(x * (1 + i))
+                g.replay()
+    torch.cuda.synchronize()
+    for i, (g, xi, yi, st) in enumerate(graphs):
+        assert torch.equal(yi, int4_linear(int4_linear(x * (1 + i), w, s)[:, :512].repeat(1, 2), w, s))
+
+
+def test_modules():
+    from llms_b200.kernels import Int4FFN, Int4Linear, int4_fused_gate_up_silu
+    from llms_b200.qwen3 import FFN
+    ffn = FFN(256, 384).to("cuda", BF)
+    m, lin = Int4FFN.from_eager(ffn, group=64), Int4Linear.from_linear(ffn.down, group=128)
+    x, h = _x(3, 256, BF), _x(2, 384, BF)
+    with torch.inference_mode():
+        y = int4_fused_gate_up_silu(x, m.wg, m.sg, m.wu, m.su)
+        _check_gate(y, x, m.wg, m.sg, m.wu, m.su)
+        assert torch.equal(m(x), ffn.down(y))
+        _check_linear(lin(h), h, lin.qweight, lin.scale)
