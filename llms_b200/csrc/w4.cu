@@ -17,9 +17,12 @@
 //     the weights 4 apart in a 32-bit word;
 //   * a group's products are summed in fp32 in accumulators of their own, which
 //     its scale then joins to the row's: no product is rounded;
-//   * K is split over a cluster of CTAs with 128 weight rows each, and the
-//     partial sums meet in distributed shared memory: no workspace, no atomics;
 //   * before griddepcontrol.wait a CTA only asks for its first weights in L2.
+// Up to 16 rows of x, one persistent CTA per SM walks tiles of 16 weight rows.
+// Its warps split K; each has the part of x that it needs in registers (or, for
+// long K, x lies in shared memory) and fills a ring of its own with cp.async,
+// several tiles ahead, so only the sums of a tile meet at a barrier.  Otherwise K is split over a cluster of CTAs with 128 weight rows
+// each, and the sums meet in distributed shared memory.
 // More rows run in chunks of 64, or, from kDenseRows on, the weights
 // are expanded to 16 bits (rounded once: the tcgen05 GEMM's operands are
 // 16-bit) into the caller's workspace and the dense GEMM takes them.
@@ -79,6 +82,12 @@ template <> struct Nib<__half> {
   }
 };
 
+// 8 values of x in the order of a word's pairs: 0 4 1 5 2 6 3 7
+__device__ __forceinline__ uint4 pair_order(const uint4& v) {
+  return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                    __byte_perm(v.y, v.w, 0x7632));
+}
+
 // First column (inside a chunk) of the 8 weights that lane c of a row holds in
 // word j after spread(): words j of the four lanes lie in one group.
 template <int G>
@@ -115,6 +124,253 @@ __device__ __forceinline__ void spread(uint32_t (&w)[4], int c) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// persistent kernel: M <= 8 MT rows of x
+// ---------------------------------------------------------------------------
+constexpr int kStreamWarps = 16;    // at most
+constexpr int kSlice = 2 * kChunk;  // columns per warp and step: 128 bytes of a row
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {  // zeros where not ok
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Ring slots per warp (2 KB of each matrix a slot).
+__host__ __device__ constexpr int stream_depth(bool gate, bool xreg) { return (xreg ? 6 : 4) / (gate ? 2 : 1); }
+
+// XREG: every warp has one slice of K, and its part of x stays in registers;
+// otherwise all of x is staged in shared memory.
+template <typename T, int MT, int G, bool GATE, bool XREG>
+__global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const __grid_constant__ W4Params p) {
+  constexpr int NM = GATE ? 2 : 1;
+  constexpr int D = stream_depth(GATE, XREG);
+  constexpr int GPC = kChunk / G;  // groups per chunk
+  constexpr int WPG = 4 / GPC;     // words of a lane per group
+  constexpr int SPL = G == 32 ? 2 : 1;  // scales of a slice per lane (4 lanes share a row)
+  constexpr uint32_t MAT = 16 * 128;    // bytes of a slot, one matrix
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  const int r = lane >> 2, c = lane & 3;
+  const int M = p.M, N = p.N, K = p.K;
+  const int nsl = (K + kSlice - 1) / kSlice;
+  const int per = XREG ? 1 : (nsl + nw - 1) / nw;  // slices of a tile per warp: warp + nw i
+  const int ntiles = (N + 15) / 16;
+  const int mine = (ntiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // tiles blockIdx.x + i gridDim.x
+  const int total = mine * per;
+
+  unsigned char* ring = smem_raw + (size_t)warp * D * NM * MAT;
+  const uint32_t ring_u = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  float* red = reinterpret_cast<float*>(smem_raw + (size_t)nw * D * NM * MAT);  // [NM][warp][16][rp]
+  const int rp = (M + 1) & ~1;
+  T* xs = reinterpret_cast<T*>(red + NM * nw * 16 * rp);                        // [M][xpitch]
+  const int xpitch = nsl * kSlice + 32;  // rows of x 64 bytes apart in the banks
+
+  // ---- the load cursor ----
+  int lt = blockIdx.x, li = 0, lit = 0;  // tile, slice number of the warp, item
+  const int crow = lane >> 3, cpos = lane & 7;  // a copy takes 4 rows of 8 x 16 bytes
+  // odd rows with their halves swapped: a fragment load takes 64 bytes of an even and of an odd row
+  const uint32_t cdst = ring_u + crow * 128 + ((cpos ^ ((crow & 1) << 2)) << 4);
+  float sv[D][NM][2][SPL];
+  auto load = [&](int u) {
+    const int sl = warp + nw * li;
+    if (lit < total && sl < nsl) {
+      const int kb = sl * (kSlice / 2) + cpos * 16;  // byte of the row
+      const int row0 = lt * 16 + crow;
+#pragma unroll
+      for (int mtx = 0; mtx < NM; ++mtx) {
+        const uint8_t* src = p.w[mtx] + (int64_t)row0 * p.ldw + kb;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool ok = row0 + 4 * i < N && kb < (K >> 1);
+          cp_async16(cdst + (u * NM + mtx) * MAT + i * 512, ok ? src : p.w[mtx], ok);
+          src += 4 * p.ldw;
+        }
+      }
+      const int g0 = sl * (kSlice / G) + (G == 128 ? c & 1 : c);
+#pragma unroll
+      for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = lt * 16 + r + 8 * h;
+          const T* s = static_cast<const T*>(p.s[mtx]) + (int64_t)row * p.lds + g0;
+#pragma unroll
+          for (int q = 0; q < SPL; ++q)
+            sv[u][mtx][h][q] = row < N && (g0 + 4 * q) * G < K ? to_f<T>(s[4 * q]) : 0.f;
+        }
+    }
+    cp_commit();
+    ++lit;
+    if (++li == per) {
+      li = 0;
+      lt += gridDim.x;
+    }
+  };
+  {  // the first slices on their way to L2 (nothing is read before the wait)
+    int t = blockIdx.x, i = 0;
+#pragma unroll
+    for (int u = 0; u < D; ++u) {
+      const int kb = (warp + nw * i) * (kSlice / 2);
+      if (lane < 16 && u < total && t * 16 + lane < N && kb < (K >> 1))
+#pragma unroll
+        for (int mtx = 0; mtx < NM; ++mtx) prefetch_l2(p.w[mtx] + (int64_t)(t * 16 + lane) * p.ldw + kb);
+      if (++i == per) {
+        i = 0;
+        t += gridDim.x;
+      }
+    }
+  }
+  pdl_trigger();
+  pdl_wait();
+#pragma unroll
+  for (int u = 0; u < D; ++u) load(u);
+
+  // ---- x, zero past M and K, in the order of the pairs 0 4 1 5 2 6 3 7 ----
+  const T* x = static_cast<const T*>(p.x);
+  uint4 xr[XREG ? 2 : 1][4][MT];  // of the warp's slice: chunk, word, n-tile
+  if constexpr (XREG) {
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const int k = warp * kSlice + hh * kChunk + word_col<G>(j, c), m = r + 8 * t;
+          xr[hh][j][t] = m < M && k < K ? pair_order(*reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k))
+                                        : make_uint4(0, 0, 0, 0);
+        }
+  } else {
+    // 8 columns from word_col(j, c) lie at 16-byte place 4 j + c of their chunk
+    const int words = nsl * (kSlice / 8);
+    for (int i = threadIdx.x; i < M * words; i += blockDim.x) {
+      const int m = i / words, wd = i - m * words;
+      const int place = wd % 16, ch = wd / 16;
+      const int k = ch * kChunk + word_col<G>(place / 4, place % 4);
+      *reinterpret_cast<uint4*>(xs + (int64_t)m * xpitch + ch * kChunk + place * 8) =
+          k < K ? pair_order(*reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k)) : make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+  }
+
+  float acc[NM][MT][4];
+  auto clear = [&]() {
+#pragma unroll
+    for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mtx][t][e] = 0.f;
+  };
+  clear();
+  const uint32_t frag = ring_u + r * 128 + ((c ^ ((r & 1) << 2)) << 4);
+  int i = 0, tile = blockIdx.x;  // of the item: its number in the tile, the tile
+  for (int it0 = 0; it0 < total; it0 += D) {
+#pragma unroll
+    for (int u = 0; u < D; ++u) {
+      if (it0 + u >= total) break;
+      const int sl = warp + nw * i;
+      cp_wait<D - 1>();
+      __syncwarp();
+      if (sl < nsl) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t wd[NM][2][4];
+#pragma unroll
+          for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t at = (frag ^ (hh << 6)) + (u * NM + mtx) * MAT + h * 1024;
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                           : "=r"(wd[mtx][h][0]), "=r"(wd[mtx][h][1]), "=r"(wd[mtx][h][2]), "=r"(wd[mtx][h][3])
+                           : "r"(at) : "memory");
+              spread<G>(wd[mtx][h], c);
+            }
+#pragma unroll
+          for (int g = 0; g < GPC; ++g) {
+            float part[NM][MT][4];
+#pragma unroll
+            for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+              for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[mtx][t][e] = 0.f;
+#pragma unroll
+            for (int jj = 0; jj < WPG; ++jj) {
+              const int j = g * WPG + jj;
+              uint4 b[MT];
+#pragma unroll
+              for (int t = 0; t < MT; ++t) {
+                if constexpr (XREG) {
+                  b[t] = xr[hh][j][t];
+                } else {
+                  b[t] = make_uint4(0, 0, 0, 0);
+                  if (r + 8 * t < M)
+                    b[t] = *reinterpret_cast<const uint4*>(xs + (int64_t)(r + 8 * t) * xpitch + sl * kSlice + hh * kChunk + 32 * j + 8 * c);
+                }
+              }
+#pragma unroll
+              for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const uint32_t a[4] = {Nib<T>::pair(wd[mtx][0][j], 2 * q), Nib<T>::pair(wd[mtx][1][j], 2 * q),
+                                         Nib<T>::pair(wd[mtx][0][j], 2 * q + 1), Nib<T>::pair(wd[mtx][1][j], 2 * q + 1)};
+#pragma unroll
+                  for (int t = 0; t < MT; ++t) Nib<T>::mma(part[mtx][t], a, q ? b[t].z : b[t].x, q ? b[t].w : b[t].y);
+                }
+            }
+            const int gi = hh * GPC + g;  // the group in the slice: held by lane gi % 4 of the row
+#pragma unroll
+            for (int mtx = 0; mtx < NM; ++mtx) {
+              const float s0 = __shfl_sync(0xffffffffu, sv[u][mtx][0][gi / 4], (lane & 28) + gi % 4);
+              const float s1 = __shfl_sync(0xffffffffu, sv[u][mtx][1][gi / 4], (lane & 28) + gi % 4);
+#pragma unroll
+              for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[mtx][t][e] = fmaf(part[mtx][t][e], e < 2 ? s0 : s1, acc[mtx][t][e]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      load(u);
+      if (++i == per) {  // the tile's sums meet
+        i = 0;
+        __syncthreads();  // (the last tile's are read)
+#pragma unroll
+        for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (8 * t + 2 * c < M)
+                *reinterpret_cast<float2*>(red + ((mtx * nw + warp) * 16 + r + 8 * h) * rp + 8 * t + 2 * c) =
+                    make_float2(acc[mtx][t][2 * h], acc[mtx][t][2 * h + 1]);
+        clear();
+        __syncthreads();
+        for (int o = threadIdx.x; o < 16 * M; o += blockDim.x) {
+          const int row = o % 16, m = o / 16, n = tile * 16 + row;
+          float v[NM];
+#pragma unroll
+          for (int mtx = 0; mtx < NM; ++mtx) {
+            v[mtx] = 0.f;
+            for (int w = 0; w < nw; ++w) v[mtx] += red[((mtx * nw + w) * 16 + row) * rp + m];
+          }
+          if (n < N) static_cast<T*>(p.y)[(int64_t)m * p.ldy + n] = from_f<T>(GATE ? silu_mul(v[0], v[NM - 1]) : v[0]);
+        }
+        tile += gridDim.x;
+      }
+    }
+  }
+  cp_wait<0>();
+}
+
+// ---------------------------------------------------------------------------
+// cluster kernel
+// ---------------------------------------------------------------------------
 // MT: n-tiles of 8 rows of x; CS: CTAs of a cluster (K split).
 template <typename T, int MT, int G, bool GATE, int CS>
 __global__ void __launch_bounds__(kThreads) w4_kernel(const __grid_constant__ W4Params p) {
@@ -189,15 +445,9 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const __grid_constant__ W4
       const int m = i / words, wd = i - m * words;
       const int place = wd % 16, ch = wd / 16;
       const int k = k_begin + ch * kChunk + word_col<G>(place / 4, place % 4);
-      uint32_t o[4] = {0, 0, 0, 0};
-      if (m < p.M && k < k_end) {
-        const uint4 v = *reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k);
-        o[0] = __byte_perm(v.x, v.z, 0x5410);
-        o[1] = __byte_perm(v.x, v.z, 0x7632);
-        o[2] = __byte_perm(v.y, v.w, 0x5410);
-        o[3] = __byte_perm(v.y, v.w, 0x7632);
-      }
-      *reinterpret_cast<uint4*>(xs + (int64_t)m * xpitch + ch * kChunk + place * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(xs + (int64_t)m * xpitch + ch * kChunk + place * 8) =
+          m < p.M && k < k_end ? pair_order(*reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k))
+                               : make_uint4(0, 0, 0, 0);
     }
   }
   __syncthreads();
@@ -326,10 +576,45 @@ size_t smem_bytes(int MT, bool gate, int kslice) {
   return (size_t)MP * (kslice + 32) * 2 + (size_t)(gate ? 2 : 1) * kRows * (MP + 2) * sizeof(float);
 }
 constexpr size_t kMaxSmem = 220 * 1024;
+constexpr size_t kStreamSmem = 226 * 1024;
 
 int kslice_of(int K, int cs) {
   const int per = (K + cs - 1) / cs;
   return (per + kChunk - 1) / kChunk * kChunk;
+}
+
+// Warps of the persistent kernel: as few as take the slices in as many rounds as 16 would.
+int stream_warps(int K) {
+  const int nsl = (K + kSlice - 1) / kSlice, rounds = (nsl + kStreamWarps - 1) / kStreamWarps;
+  return (nsl + rounds - 1) / rounds;
+}
+bool stream_xreg(int K) { return (K + kSlice - 1) / kSlice <= kStreamWarps; }
+size_t stream_smem(int M, int K, bool gate) {
+  const int nm = gate ? 2 : 1, nw = stream_warps(K), nsl = (K + kSlice - 1) / kSlice;
+  const bool xreg = stream_xreg(K);
+  return (size_t)nw * stream_depth(gate, xreg) * nm * 2048 + sizeof(float) * nm * nw * 16 * ((M + 1) & ~1) +
+         (xreg ? 0 : (size_t)M * (nsl * kSlice + 32) * 2);
+}
+bool stream_fits(int M, int K, bool gate) {
+  return M <= 16 && (M <= 8 || stream_xreg(K)) && stream_smem(M, K, gate) <= kStreamSmem;
+}
+
+template <typename T, int MT, int G, bool GATE, bool XREG>
+int launch_stream(const W4Params& p, cudaStream_t st) {
+  auto kern = w4_stream_kernel<T, MT, G, GATE, XREG>;
+  static bool configured[64] = {false};
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return B200MM_ERR_DEVICE;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kStreamSmem) != cudaSuccess)
+      return B200MM_ERR_LAUNCH;
+    configured[dev] = true;
+  }
+  const int tiles = (p.N + 15) / 16, sms = num_sms(dev);
+  return launch_pdl(kern, dim3(tiles < sms ? tiles : sms), dim3(32 * stream_warps(p.K)), stream_smem(p.M, p.K, GATE), st,
+                    p) == cudaSuccess
+             ? B200MM_OK
+             : B200MM_ERR_LAUNCH;
 }
 
 template <typename T, int MT, int G, bool GATE, int CS>
@@ -337,13 +622,13 @@ int launch_w4(const W4Params& p, cudaStream_t st) {
   auto kern = w4_kernel<T, MT, G, GATE, CS>;
   const size_t smem = smem_bytes(MT, GATE, p.kslice);
   if (smem > kMaxSmem) return B200MM_ERR_SHAPE;
-  static int configured[64] = {0};
+  static bool configured[64] = {false};
   const int dev = current_device();
   if (dev < 0 || dev >= 64) return B200MM_ERR_DEVICE;
-  if ((int)smem > configured[dev]) {
+  if (!configured[dev]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem) != cudaSuccess)
       return B200MM_ERR_LAUNCH;
-    configured[dev] = (int)kMaxSmem;
+    configured[dev] = true;
   }
   const int groups = (p.N + kRows - 1) / kRows;
   return launch_pdl_cluster(kern, dim3(groups * CS), dim3(kThreads), smem, st, CS, p) == cudaSuccess ? B200MM_OK
@@ -352,6 +637,14 @@ int launch_w4(const W4Params& p, cudaStream_t st) {
 
 template <typename T, int MT, int G>
 int launch_gate(const W4Params& p, bool gate, cudaStream_t st) {
+  if constexpr (MT <= 2) {
+    if (stream_fits(p.M, p.K, gate)) {
+      if (stream_xreg(p.K))
+        return gate ? launch_stream<T, MT, G, true, true>(p, st) : launch_stream<T, MT, G, false, true>(p, st);
+      if constexpr (MT == 1)
+        return gate ? launch_stream<T, 1, G, true, false>(p, st) : launch_stream<T, 1, G, false, false>(p, st);
+    }
+  }
   return gate ? launch_w4<T, MT, G, true, 8>(p, st) : launch_w4<T, MT, G, false, 8>(p, st);
 }
 template <typename T, int MT>

@@ -49,33 +49,37 @@ def _check_w4(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, name: str) -> i
     """The group size of ``w``, ``s``; raises where they do not fit ``x`` or each other."""
     if w.dim() != 2 or w.dtype != torch.uint8:
         raise ValueError(f"{name} must be a 2D uint8 tensor (N, K / 2), got {w.dtype} {tuple(w.shape)}")
-    N, K = w.shape[0], 2 * w.shape[1]
+    N, K = w.shape
+    K *= 2
     if x.shape[-1] != K:
         raise ValueError(f"x last dim {x.shape[-1]} != {name}'s K {K}")
-    if s.dim() != 2 or s.shape[0] != N or s.shape[1] < 1 or K // s.shape[1] not in GROUPS or K % s.shape[1]:
+    groups = s.shape[1] if s.dim() == 2 else 0
+    if not groups or s.shape[0] != N or K % groups or K // groups not in GROUPS:
         raise ValueError(f"{name} scales must be ({N}, {K} / group) with group one of {GROUPS}, got {tuple(s.shape)}")
-    if x.dtype not in (torch.bfloat16, torch.float16) or s.dtype != x.dtype:
-        raise ValueError(f"x ({x.dtype}) and {name} scales ({s.dtype}) must share a dtype, bfloat16 or float16")
-    if x.device != w.device or x.device != s.device:
-        raise ValueError(f"x ({x.device}), {name} ({w.device}), scales ({s.device}) must be on the same device")
-    return K // s.shape[1]
+    dtype, device = x.dtype, x.device
+    if dtype not in (torch.bfloat16, torch.float16) or s.dtype != dtype:
+        raise ValueError(f"x ({dtype}) and {name} scales ({s.dtype}) must share a dtype, bfloat16 or float16")
+    if device != w.device or device != s.device:
+        raise ValueError(f"x ({device}), {name} ({w.device}), scales ({s.device}) must be on the same device")
+    return K // groups
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """2-D ``t`` with unit inner stride on 16-byte rows (copied if it is not)."""
-    size = t.element_size()
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * size % 16 == 0 and t.stride(0) >= t.shape[1]:
+    ld, inner = t.stride()
+    if inner == 1 and not (t.data_ptr() | ld * t.element_size()) & 15 and ld >= t.shape[1]:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _scales(s: torch.Tensor) -> torch.Tensor:
-    return s if s.stride(1) == 1 and s.stride(0) >= s.shape[1] else s.contiguous()
+    ld, inner = s.stride()
+    return s if inner == 1 and ld >= s.shape[1] else s.contiguous()
 
 
-def _workspace(M: int, N: int, K: int, gate: int, device: torch.device) -> torch.Tensor | None:
+def _workspace(x: torch.Tensor, M: int, N: int, K: int, gate: int) -> tuple[torch.Tensor | None, int]:
     need = _capi.lib.b200mm_w4_workspace_size(M, N, K, gate) if M > 64 else 0
-    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    return (x.new_empty(need, dtype=torch.uint8) if need else None), need
 
 
 def int4_linear(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
@@ -89,19 +93,16 @@ def int4_linear(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor) -> torch.Tens
     """
     group = _check_w4(x, w, s, "W")
     N, K = w.shape[0], x.shape[-1]
-    x2 = x.reshape(-1, K)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
     M = x2.shape[0]
-    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], N))
     if M and N:
         _capi.require_cuda(x)
         x2, w, s = _rows16(x2), _rows16(w), _scales(s)
-        with _capi.on_device(x):
-            ws = _workspace(M, N, K, 0, x.device)
-            st = _capi.lib.b200mm_linear_w4(
-                x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), s.data_ptr(), s.stride(0), group,
-                y.data_ptr(), N, M, N, K, _capi.dtype_code(x.dtype), None if ws is None else ws.data_ptr(),
-                0 if ws is None else ws.numel(), _capi.stream_of(x))
-        _capi.check(st, "b200mm_linear_w4")
+        ws, nb = _workspace(x, M, N, K, 0)
+        _capi.launch("b200mm_linear_w4", x, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), s.data_ptr(),
+                     s.stride(0), group, y.data_ptr(), N, M, N, K, _capi.DTYPE_CODES[x.dtype],
+                     None if ws is None else ws.data_ptr(), nb)
     return y
 
 
@@ -120,9 +121,9 @@ def int4_fused_gate_up_silu(x: torch.Tensor, wg: torch.Tensor, sg: torch.Tensor,
     group = _check_w4(x, wg, sg, "Wg")
     _check_w4(x, wu, su, "Wu")
     N, K = wg.shape[0], x.shape[-1]
-    x2 = x.reshape(-1, K)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
     M = x2.shape[0]
-    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], N))
     if M and N:
         _capi.require_cuda(x)
         x2, wg, wu, sg, su = _rows16(x2), _rows16(wg), _rows16(wu), _scales(sg), _scales(su)
@@ -130,13 +131,10 @@ def int4_fused_gate_up_silu(x: torch.Tensor, wg: torch.Tensor, sg: torch.Tensor,
             wg, wu = wg.contiguous(), wu.contiguous()
         if sg.stride(0) != su.stride(0):
             sg, su = sg.contiguous(), su.contiguous()
-        with _capi.on_device(x):
-            ws = _workspace(M, N, K, 1, x.device)
-            st = _capi.lib.b200mm_gate_up_silu_w4(
-                x2.data_ptr(), x2.stride(0), wg.data_ptr(), wu.data_ptr(), wg.stride(0), sg.data_ptr(), su.data_ptr(),
-                sg.stride(0), group, y.data_ptr(), N, M, N, K, _capi.dtype_code(x.dtype),
-                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _capi.stream_of(x))
-        _capi.check(st, "b200mm_gate_up_silu_w4")
+        ws, nb = _workspace(x, M, N, K, 1)
+        _capi.launch("b200mm_gate_up_silu_w4", x, x2.data_ptr(), x2.stride(0), wg.data_ptr(), wu.data_ptr(),
+                     wg.stride(0), sg.data_ptr(), su.data_ptr(), sg.stride(0), group, y.data_ptr(), N, M, N, K,
+                     _capi.DTYPE_CODES[x.dtype], None if ws is None else ws.data_ptr(), nb)
     return y
 
 

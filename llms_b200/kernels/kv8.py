@@ -118,9 +118,9 @@ def _pos(pos, B: int, device: torch.device):
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with a contiguous last dim on 16-byte rows (copied if it is not)."""
-    per = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % per for s in t.stride()[:-1]):
+    """4-D ``t`` with a contiguous last dim on 16-byte rows (copied if it is not)."""
+    b, h, n, d = t.stride()
+    if d == 1 and not ((b | h | n) * t.element_size() | t.data_ptr()) & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -158,11 +158,8 @@ def int8_kv_append(kv: Int8KV, k: torch.Tensor, v: torch.Tensor, pos: int | torc
     if k.numel() == 0:
         return
     k, v = _aligned(k), _aligned(v)
-    with _capi.on_device(k):
-        st = _capi.lib.b200mm_kv8_append(
-            kv._ref, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-            v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), B, T, host, dev, stride, _capi.stream_of(k))
-    _capi.check(st, "b200mm_kv8_append")
+    _capi.launch("b200mm_kv8_append", k, kv._ref, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, T,
+                 host, dev, stride)
 
 
 def int8_kv_expand(kv: Int8KV, length: int, *, batch: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -173,12 +170,9 @@ def int8_kv_expand(kv: Int8KV, length: int, *, batch: int | None = None) -> tupl
         raise ValueError(f"length {length}, batch {B} do not fit a cache of {tuple(kv.kq.shape)}")
     _capi.require_cuda(kv.kq)
     shape = (B, kv.num_kv_heads, length, kv.head_dim)
-    k, v = (torch.empty(shape, dtype=kv.dtype, device=kv.device) for _ in range(2))
+    k, v = kv.kt.new_empty(shape), kv.kt.new_empty(shape)
     if k.numel():
-        with _capi.on_device(k):
-            st = _capi.lib.b200mm_kv8_expand(kv._ref, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                                             B, length, _capi.stream_of(k))
-        _capi.check(st, "b200mm_kv8_expand")
+        _capi.launch("b200mm_kv8_expand", k, kv._ref, k.data_ptr(), v.data_ptr(), *k.stride()[:3], B, length)
     return k, v
 
 
@@ -193,13 +187,14 @@ def _check_query(kv: Int8KV, q: torch.Tensor) -> None:
     _capi.require_cuda(q)
 
 
-def _workspace(kv: Int8KV, B: int, H: int) -> torch.Tensor | None:
+def _workspace(kv: Int8KV, B: int, H: int) -> tuple[torch.Tensor | None, int]:
     """A call's own workspace, from the caching allocator (so ordered by the
     current stream, and private to the graph that a call is captured into)."""
     need = kv._ws.get((B, H))
     if need is None:
-        need = kv._ws[(B, H)] = _capi.lib.b200mm_kv8_decode_workspace_size(kv._ref, B, H)
-    return torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
+        with _capi.on_device(kv.kq):
+            need = kv._ws[(B, H)] = _capi.lib.b200mm_kv8_decode_workspace_size(kv._ref, B, H)
+    return (kv.kq.new_empty(need, dtype=torch.uint8) if need else None), need
 
 
 def int8_kv_decode_attn(q: torch.Tensor, kv: Int8KV, pos: int | torch.Tensor, *, scale: float) -> torch.Tensor:
@@ -218,16 +213,13 @@ def int8_kv_decode_attn(q: torch.Tensor, kv: Int8KV, pos: int | torch.Tensor, *,
     _check_host_pos(kv, pos, 1)
     B, H, _, D = q.shape
     host, dev, stride = _pos(pos, B, kv.device)
-    out = torch.empty((B, H, 1, D), dtype=q.dtype, device=q.device)
+    out = q.new_empty((B, H, 1, D))
     if B == 0:
         return out
     q = _aligned(q)
-    with _capi.on_device(q):
-        ws = _workspace(kv, B, H)
-        st = _capi.lib.b200mm_kv8_decode(
-            kv._ref, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), H * D, D, B, H, host, dev, stride,
-            float(scale), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _capi.stream_of(q))
-    _capi.check(st, "b200mm_kv8_decode")
+    ws, nb = _workspace(kv, B, H)
+    _capi.launch("b200mm_kv8_decode", q, kv._ref, q.data_ptr(), *q.stride()[:2], out.data_ptr(), H * D, D, B, H, host, dev,
+                 stride, scale, None if ws is None else ws.data_ptr(), nb)
     return out
 
 
@@ -243,17 +235,14 @@ def int8_kv_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: Int8KV, 
         raise ValueError(f"k {tuple(k.shape)} must hold one token for each of q's {B} rows")
     _check_host_pos(kv, pos, 1)
     host, dev, stride = _pos(pos, B, kv.device)
-    out = torch.empty((B, H, 1, D), dtype=q.dtype, device=q.device)
+    out = q.new_empty((B, H, 1, D))
     if B == 0:
         return out
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    with _capi.on_device(q):
-        ws = _workspace(kv, B, H)
-        st = _capi.lib.b200mm_kv8_step(
-            kv._ref, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), H * D, D, B, H, host, dev, stride, float(scale),
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _capi.stream_of(q))
-    _capi.check(st, "b200mm_kv8_step")
+    ws, nb = _workspace(kv, B, H)
+    _capi.launch("b200mm_kv8_step", q, kv._ref, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+                 *v.stride()[:2], out.data_ptr(), H * D, D, B, H, host, dev, stride, scale,
+                 None if ws is None else ws.data_ptr(), nb)
     return out
 
 

@@ -47,20 +47,15 @@ def b200_token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int 
         raise ValueError(f"top must be in 0..{min(V, MAX_TOP)}, got {top}")
     code = _capi.dtype_code(logits.dtype)
     _capi.require_cuda(logits)
-    x = logits.reshape(-1, V)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if x.stride(-1) != 1 or x.stride(0) < V:
         x = x.contiguous()
     M = x.shape[0]
     lead = logits.shape[:-1]
-    both = torch.empty((2, *lead), dtype=torch.float32, device=x.device)
-    ids = torch.empty((*lead, top), dtype=torch.int64, device=x.device)
-    lps = torch.empty((*lead, top), dtype=torch.float32, device=x.device)
-    out = TokenLogprobs(both[0], both[1], ids, lps)
+    lp, ent = x.new_empty((2, *lead), dtype=torch.float32).unbind()
+    ids, lps = x.new_empty((*lead, top), dtype=torch.int64), x.new_empty((*lead, top), dtype=torch.float32)
     if M:
         toks = tokens.contiguous()
-        with _capi.on_device(x):
-            st = _capi.lib.b200mm_token_logprobs(
-                x.data_ptr(), x.stride(0), toks.data_ptr(), both.data_ptr(), both.data_ptr() + 4 * M, ids.data_ptr(),
-                lps.data_ptr(), M, V, top, code, _capi.stream_of(x))
-        _capi.check(st, "b200mm_token_logprobs")
-    return out
+        _capi.launch("b200mm_token_logprobs", x, x.data_ptr(), x.stride(0), toks.data_ptr(), lp.data_ptr(), ent.data_ptr(),
+                     ids.data_ptr(), lps.data_ptr(), M, V, top, code)
+    return TokenLogprobs(lp, ent, ids, lps)
