@@ -142,10 +142,69 @@ __device__ __forceinline__ void cp_wait() {
 // Ring slots per warp (2 KB of each matrix a slot).
 __host__ __device__ constexpr int stream_depth(bool gate, bool xreg) { return (xreg ? 6 : 4) / (gate ? 2 : 1); }
 
+// The eight weights of a word as four fp16 pairs, (0, 4), (1, 5), (2, 6), (3, 7):
+// under the exponent of 2^10 a low half is 1024 + u, a high half 1024 + 16 u, so
+// one shift serves two logic instructions (bf16's 7 bits would want one each).
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(mask), "r"(bits));
+  return v;
+}
+__device__ __forceinline__ void nibbles_h2(uint32_t w, uint32_t (&o)[4]) {
+  const __half2 low = __float2half2_rn(-1032.f), k = __float2half2_rn(0.0625f), high = __float2half2_rn(-72.f);
+  uint32_t v[4] = {and_or(w, 0x000f000fu, 0x64006400u), and_or(w, 0x00f000f0u, 0x64006400u),
+                   and_or(w >> 8, 0x000f000fu, 0x64006400u), and_or(w >> 8, 0x00f000f0u, 0x64006400u)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&v[i]);
+    const __half2 q = i & 1 ? __hfma2(h, k, high) : __hadd2(h, low);
+    o[i] = *reinterpret_cast<const uint32_t*>(&q);
+  }
+}
+
+// Eight values of x as fp16, times `up` (bf16; fp16 as they are), in the order of a word's pairs.
+template <typename T>
+__device__ __forceinline__ uint4 x_pairs(const uint4& v, float up) {
+  if constexpr (std::is_same<T, __half>::value) return pair_order(v);
+  float f[8];
+  Chunk<T>::unpack(v, f);
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(f[i] * up, f[i + 4] * up);
+    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+template <typename T>
+__device__ __forceinline__ float x_max(const uint4& v) {
+  float f[8], m = 0.f;
+  Chunk<T>::unpack(v, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
+  return m;
+}
+// The power of two that brings `mx` into [2^14, 2^15), and its inverse (both normal).
+__device__ __forceinline__ float x_up(float mx, float& down) {
+  const int e = max(1, min(268 - (int)(__float_as_uint(mx) >> 23), 253));
+  down = __uint_as_float((uint32_t)(254 - e) << 23);
+  return __uint_as_float((uint32_t)e << 23);
+}
+
+template <typename T>
+__device__ __forceinline__ float scale_of(uint32_t bits) {
+  const unsigned short h = (unsigned short)bits;
+  return to_f<T>(*reinterpret_cast<const T*>(&h));
+}
+
+// Products are fp16 x fp16: bf16 rows of x are scaled by a power of two per
+// slice of K that brings the largest element into [2^14, 2^15), so they are
+// exact down to 2^-29 of it and within 2^-39 of it below; the sums are scaled back.
 // XREG: every warp has one slice of K, and its part of x stays in registers;
 // otherwise all of x is staged in shared memory.
 template <typename T, int MT, int G, bool GATE, bool XREG>
 __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const __grid_constant__ W4Params p) {
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int NM = GATE ? 2 : 1;
   constexpr int D = stream_depth(GATE, XREG);
   constexpr int GPC = kChunk / G;  // groups per chunk
@@ -167,47 +226,71 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
   const uint32_t ring_u = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   float* red = reinterpret_cast<float*>(smem_raw + (size_t)nw * D * NM * MAT);  // [NM][warp][16][rp]
   const int rp = (M + 1) & ~1;
-  T* xs = reinterpret_cast<T*>(red + NM * nw * 16 * rp);                        // [M][xpitch]
   const int xpitch = nsl * kSlice + 32;  // rows of x 64 bytes apart in the banks
+  __half* xs = reinterpret_cast<__half*>(red + NM * nw * 16 * rp);             // [M][xpitch]
+  float* xdown = reinterpret_cast<float*>(xs + (XREG ? 0 : (int64_t)M * xpitch));  // [nsl][8]: 1 / the slices' powers of two
 
-  // ---- the load cursor ----
+  // ---- the load cursor: lane (r, c) takes 16 bytes at 16 c and 64 + 16 c of rows r and r + 8 ----
   int lt = blockIdx.x, li = 0, lit = 0;  // tile, slice number of the warp, item
-  const int crow = lane >> 3, cpos = lane & 7;  // a copy takes 4 rows of 8 x 16 bytes
+  const int64_t tile_step = (int64_t)gridDim.x * 16;
+  const uint8_t* wsrc[NM];
+  const T* ssrc[NM];
+#pragma unroll
+  for (int mtx = 0; mtx < NM; ++mtx) {
+    const int64_t row = (int64_t)blockIdx.x * 16 + r;
+    wsrc[mtx] = p.w[mtx] + row * p.ldw + warp * (kSlice / 2) + 16 * c;
+    ssrc[mtx] = static_cast<const T*>(p.s[mtx]) + row * p.lds + warp * (kSlice / G) + (G == 128 ? c & 1 : c);
+  }
   // odd rows with their halves swapped: a fragment load takes 64 bytes of an even and of an odd row
-  const uint32_t cdst = ring_u + crow * 128 + ((cpos ^ ((crow & 1) << 2)) << 4);
-  float sv[D][NM][2][SPL];
+  const uint32_t frag = ring_u + r * 128 + ((c ^ ((r & 1) << 2)) << 4);
+  uint32_t sv[D][NM][2][SPL];  // scales as they are: converting them here would wait for them
+  auto raw = [](const T* q) -> uint32_t { return *reinterpret_cast<const unsigned short*>(q); };
   auto load = [&](int u) {
-    const int sl = warp + nw * li;
-    if (lit < total && sl < nsl) {
-      const int kb = sl * (kSlice / 2) + cpos * 16;  // byte of the row
-      const int row0 = lt * 16 + crow;
+    const int k0 = (warp + nw * li) * kSlice;
+    if (lit < total && k0 < K) {
+      const int row = lt * 16 + r;
+      if (lt * 16 + 16 <= N && k0 + kSlice <= K) {
 #pragma unroll
-      for (int mtx = 0; mtx < NM; ++mtx) {
-        const uint8_t* src = p.w[mtx] + (int64_t)row0 * p.ldw + kb;
+        for (int mtx = 0; mtx < NM; ++mtx) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool ok = row0 + 4 * i < N && kb < (K >> 1);
-          cp_async16(cdst + (u * NM + mtx) * MAT + i * 512, ok ? src : p.w[mtx], ok);
-          src += 4 * p.ldw;
+          for (int h = 0; h < 2; ++h) {
+            const uint8_t* src = wsrc[mtx] + (h ? 8 * p.ldw : 0);
+            const uint32_t dst = frag + (u * NM + mtx) * MAT + h * 1024;
+            cp_async16(dst, src, true);
+            cp_async16(dst ^ 64, src + 64, true);
+#pragma unroll
+            for (int q = 0; q < SPL; ++q) sv[u][mtx][h][q] = raw(ssrc[mtx] + (h ? 8 * p.lds : 0) + 4 * q);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int mtx = 0; mtx < NM; ++mtx) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint8_t* src = wsrc[mtx] + (h ? 8 * p.ldw : 0);
+            const uint32_t dst = frag + (u * NM + mtx) * MAT + h * 1024;
+            const bool in = row + 8 * h < N, a = in && k0 + 32 * c < K, b = in && k0 + kChunk + 32 * c < K;
+            cp_async16(dst, a ? src : p.w[mtx], a);
+            cp_async16(dst ^ 64, b ? src + 64 : p.w[mtx], b);
+#pragma unroll
+            for (int q = 0; q < SPL; ++q)
+              sv[u][mtx][h][q] = in && k0 + ((G == 128 ? c & 1 : c) + 4 * q) * G < K
+                                     ? raw(ssrc[mtx] + (h ? 8 * p.lds : 0) + 4 * q) : 0u;
+          }
         }
       }
-      const int g0 = sl * (kSlice / G) + (G == 128 ? c & 1 : c);
-#pragma unroll
-      for (int mtx = 0; mtx < NM; ++mtx)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = lt * 16 + r + 8 * h;
-          const T* s = static_cast<const T*>(p.s[mtx]) + (int64_t)row * p.lds + g0;
-#pragma unroll
-          for (int q = 0; q < SPL; ++q)
-            sv[u][mtx][h][q] = row < N && (g0 + 4 * q) * G < K ? to_f<T>(s[4 * q]) : 0.f;
-        }
     }
     cp_commit();
     ++lit;
-    if (++li == per) {
+    const bool wrap = ++li == per;
+    if (wrap) {
       li = 0;
       lt += gridDim.x;
+    }
+#pragma unroll
+    for (int mtx = 0; mtx < NM; ++mtx) {  // (past the last item the addresses are not used)
+      wsrc[mtx] += wrap ? tile_step * p.ldw - (int64_t)(per - 1) * nw * (kSlice / 2) : (int64_t)nw * (kSlice / 2);
+      ssrc[mtx] += wrap ? tile_step * p.lds - (int64_t)(per - 1) * nw * (kSlice / G) : (int64_t)nw * (kSlice / G);
     }
   };
   {  // the first slices on their way to L2 (nothing is read before the wait)
@@ -229,29 +312,52 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
 #pragma unroll
   for (int u = 0; u < D; ++u) load(u);
 
-  // ---- x, zero past M and K, in the order of the pairs 0 4 1 5 2 6 3 7 ----
+  // ---- x, zero past M and K ----
   const T* x = static_cast<const T*>(p.x);
   uint4 xr[XREG ? 2 : 1][4][MT];  // of the warp's slice: chunk, word, n-tile
+  float down[MT][2];              // of columns 8 t + 2 c, + 1
   if constexpr (XREG) {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
+    for (int t = 0; t < MT; ++t) {
+      const int m = r + 8 * t;
+      float mx = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const int k = warp * kSlice + hh * kChunk + word_col<G>(j, c), m = r + 8 * t;
-          xr[hh][j][t] = m < M && k < K ? pair_order(*reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k))
-                                        : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 4; ++j) {
+          const int k = warp * kSlice + hh * kChunk + word_col<G>(j, c);
+          xr[hh][j][t] = make_uint4(0, 0, 0, 0);
+          if (m < M && k < K) xr[hh][j][t] = *reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k);
+          if constexpr (BF) mx = fmaxf(mx, x_max<T>(xr[hh][j][t]));
         }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      float dn;
+      const float up = x_up(mx, dn);
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xr[hh][j][t] = x_pairs<T>(xr[hh][j][t], up);
+      down[t][0] = BF ? __shfl_sync(0xffffffffu, dn, 8 * c) : 1.f;
+      down[t][1] = BF ? __shfl_sync(0xffffffffu, dn, 8 * c + 4) : 1.f;
+    }
   } else {
-    // 8 columns from word_col(j, c) lie at 16-byte place 4 j + c of their chunk
-    const int words = nsl * (kSlice / 8);
-    for (int i = threadIdx.x; i < M * words; i += blockDim.x) {
-      const int m = i / words, wd = i - m * words;
-      const int place = wd % 16, ch = wd / 16;
-      const int k = ch * kChunk + word_col<G>(place / 4, place % 4);
-      *reinterpret_cast<uint4*>(xs + (int64_t)m * xpitch + ch * kChunk + place * 8) =
-          k < K ? pair_order(*reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k)) : make_uint4(0, 0, 0, 0);
+    // a warp per row and slice; 8 columns from word_col(j, c) lie at 16-byte place 4 j + c of their chunk
+    for (int i = warp; i < M * nsl; i += nw) {
+      const int m = i / nsl, sl = i - m * nsl;
+      const int place = lane & 15, ch = 2 * sl + (lane >> 4);
+      const int k = ch * kChunk + word_col<G>(place >> 2, place & 3);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (k < K) v = *reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k);
+      float up = 1.f;
+      if constexpr (BF) {
+        float mx = x_max<T>(v), dn;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        up = x_up(mx, dn);
+        if (lane == 0) xdown[sl * 8 + m] = dn;
+      }
+      *reinterpret_cast<uint4*>(xs + (int64_t)m * xpitch + ch * kChunk + place * 8) = x_pairs<T>(v, up);
     }
     __syncthreads();
   }
@@ -266,7 +372,6 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
         for (int e = 0; e < 4; ++e) acc[mtx][t][e] = 0.f;
   };
   clear();
-  const uint32_t frag = ring_u + r * 128 + ((c ^ ((r & 1) << 2)) << 4);
   int i = 0, tile = blockIdx.x;  // of the item: its number in the tile, the tile
   for (int it0 = 0; it0 < total; it0 += D) {
 #pragma unroll
@@ -276,6 +381,10 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
       cp_wait<D - 1>();
       __syncwarp();
       if (sl < nsl) {
+        if constexpr (!XREG) {
+          down[0][0] = BF && 2 * c < M ? xdown[sl * 8 + 2 * c] : 1.f;
+          down[0][1] = BF && 2 * c + 1 < M ? xdown[sl * 8 + 2 * c + 1] : 1.f;
+        }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           uint32_t wd[NM][2][4];
@@ -283,10 +392,9 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
           for (int mtx = 0; mtx < NM; ++mtx)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t at = (frag ^ (hh << 6)) + (u * NM + mtx) * MAT + h * 1024;
               asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                            : "=r"(wd[mtx][h][0]), "=r"(wd[mtx][h][1]), "=r"(wd[mtx][h][2]), "=r"(wd[mtx][h][3])
-                           : "r"(at) : "memory");
+                           : "r"((frag ^ (hh << 6)) + (u * NM + mtx) * MAT + h * 1024) : "memory");
               spread<G>(wd[mtx][h], c);
             }
 #pragma unroll
@@ -313,24 +421,30 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
                 }
               }
 #pragma unroll
-              for (int mtx = 0; mtx < NM; ++mtx)
+              for (int mtx = 0; mtx < NM; ++mtx) {
+                uint32_t lo[4], hi[4];
+                nibbles_h2(wd[mtx][0][j], lo);
+                nibbles_h2(wd[mtx][1][j], hi);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                  const uint32_t a[4] = {Nib<T>::pair(wd[mtx][0][j], 2 * q), Nib<T>::pair(wd[mtx][1][j], 2 * q),
-                                         Nib<T>::pair(wd[mtx][0][j], 2 * q + 1), Nib<T>::pair(wd[mtx][1][j], 2 * q + 1)};
+                  const uint32_t a[4] = {lo[2 * q], hi[2 * q], lo[2 * q + 1], hi[2 * q + 1]};
 #pragma unroll
-                  for (int t = 0; t < MT; ++t) Nib<T>::mma(part[mtx][t], a, q ? b[t].z : b[t].x, q ? b[t].w : b[t].y);
+                  for (int t = 0; t < MT; ++t) Nib<__half>::mma(part[mtx][t], a, q ? b[t].z : b[t].x, q ? b[t].w : b[t].y);
                 }
+              }
             }
             const int gi = hh * GPC + g;  // the group in the slice: held by lane gi % 4 of the row
 #pragma unroll
             for (int mtx = 0; mtx < NM; ++mtx) {
-              const float s0 = __shfl_sync(0xffffffffu, sv[u][mtx][0][gi / 4], (lane & 28) + gi % 4);
-              const float s1 = __shfl_sync(0xffffffffu, sv[u][mtx][1][gi / 4], (lane & 28) + gi % 4);
+              const float s0 = scale_of<T>(__shfl_sync(0xffffffffu, sv[u][mtx][0][gi / 4], (lane & 28) + gi % 4));
+              const float s1 = scale_of<T>(__shfl_sync(0xffffffffu, sv[u][mtx][1][gi / 4], (lane & 28) + gi % 4));
 #pragma unroll
               for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[mtx][t][e] = fmaf(part[mtx][t][e], e < 2 ? s0 : s1, acc[mtx][t][e]);
+                for (int e = 0; e < 4; ++e) {
+                  const float f = XREG || !BF ? (e < 2 ? s0 : s1) : (e < 2 ? s0 : s1) * down[t][e & 1];
+                  acc[mtx][t][e] = fmaf(part[mtx][t][e], f, acc[mtx][t][e]);
+                }
             }
           }
         }
@@ -346,9 +460,11 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
           for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              if (8 * t + 2 * c < M)
+              if (8 * t + 2 * c < M) {
+                const float d0 = XREG ? down[t][0] : 1.f, d1 = XREG ? down[t][1] : 1.f;
                 *reinterpret_cast<float2*>(red + ((mtx * nw + warp) * 16 + r + 8 * h) * rp + 8 * t + 2 * c) =
-                    make_float2(acc[mtx][t][2 * h], acc[mtx][t][2 * h + 1]);
+                    make_float2(acc[mtx][t][2 * h] * d0, acc[mtx][t][2 * h + 1] * d1);
+              }
         clear();
         __syncthreads();
         for (int o = threadIdx.x; o < 16 * M; o += blockDim.x) {
@@ -593,7 +709,7 @@ size_t stream_smem(int M, int K, bool gate) {
   const int nm = gate ? 2 : 1, nw = stream_warps(K), nsl = (K + kSlice - 1) / kSlice;
   const bool xreg = stream_xreg(K);
   return (size_t)nw * stream_depth(gate, xreg) * nm * 2048 + sizeof(float) * nm * nw * 16 * ((M + 1) & ~1) +
-         (xreg ? 0 : (size_t)M * (nsl * kSlice + 32) * 2);
+         (xreg ? 0 : (size_t)M * (nsl * kSlice + 32) * 2 + (size_t)nsl * 8 * sizeof(float));
 }
 bool stream_fits(int M, int K, bool gate) {
   return M <= 16 && (M <= 8 || stream_xreg(K)) && stream_smem(M, K, gate) <= kStreamSmem;
