@@ -203,7 +203,8 @@ __device__ __forceinline__ float scale_of(uint32_t bits) {
 // XREG: every warp has one slice of K, and its part of x stays in registers;
 // otherwise all of x is staged in shared memory.
 template <typename T, int MT, int G, bool GATE, bool XREG>
-__global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const __grid_constant__ W4Params p) {
+__global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const __grid_constant__ W4Params p, const int meet_tiles) {
+  const int meet = MT == 1 ? meet_tiles : 1;  // (16 rows: no room for more than one, nor registers to count them)
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int NM = GATE ? 2 : 1;
   constexpr int D = stream_depth(GATE, XREG);
@@ -219,15 +220,17 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
   const int nsl = (K + kSlice - 1) / kSlice;
   const int per = XREG ? 1 : (nsl + nw - 1) / nw;  // slices of a tile per warp: warp + nw i
   const int ntiles = (N + 15) / 16;
-  const int mine = (ntiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // tiles blockIdx.x + i gridDim.x
-  const int total = mine * per;
+  const int mine_tiles = (ntiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // tiles blockIdx.x + i gridDim.x
+  const int total = mine_tiles * per;
 
   unsigned char* ring = smem_raw + (size_t)warp * D * NM * MAT;
   const uint32_t ring_u = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-  float* red = reinterpret_cast<float*>(smem_raw + (size_t)nw * D * NM * MAT);  // [NM][warp][16][rp]
+  // the warps' sums of up to `meet` tiles, [tile][NM][warp][16][rp]: they meet that often
+  float* red = reinterpret_cast<float*>(smem_raw + (size_t)nw * D * NM * MAT);
   const int rp = (M + 1) & ~1;
+  const int red_n = NM * nw * 16 * rp;
   const int xpitch = nsl * kSlice + 32;  // rows of x 64 bytes apart in the banks
-  __half* xs = reinterpret_cast<__half*>(red + NM * nw * 16 * rp);             // [M][xpitch]
+  __half* xs = reinterpret_cast<__half*>(red + meet * red_n);             // [M][xpitch]
   float* xdown = reinterpret_cast<float*>(xs + (XREG ? 0 : (int64_t)M * xpitch));  // [nsl][8]: 1 / the slices' powers of two
 
   // ---- the load cursor: lane (r, c) takes 16 bytes at 16 c and 64 + 16 c of rows r and r + 8 ----
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
         for (int e = 0; e < 4; ++e) acc[mtx][t][e] = 0.f;
   };
   clear();
-  int i = 0, tile = blockIdx.x;  // of the item: its number in the tile, the tile
+  int i = 0, done = 0;  // the item's number in its tile, tiles done
   for (int it0 = 0; it0 < total; it0 += D) {
 #pragma unroll
     for (int u = 0; u < D; ++u) {
@@ -451,9 +454,9 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
       }
       __syncwarp();
       load(u);
-      if (++i == per) {  // the tile's sums meet
+      if (++i == per) {
         i = 0;
-        __syncthreads();  // (the last tile's are read)
+        float* mine = red + (done % meet) * red_n + warp * 16 * rp;
 #pragma unroll
         for (int mtx = 0; mtx < NM; ++mtx)
 #pragma unroll
@@ -462,22 +465,28 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
             for (int h = 0; h < 2; ++h)
               if (8 * t + 2 * c < M) {
                 const float d0 = XREG ? down[t][0] : 1.f, d1 = XREG ? down[t][1] : 1.f;
-                *reinterpret_cast<float2*>(red + ((mtx * nw + warp) * 16 + r + 8 * h) * rp + 8 * t + 2 * c) =
+                *reinterpret_cast<float2*>(mine + (mtx * nw * 16 + r + 8 * h) * rp + 8 * t + 2 * c) =
                     make_float2(acc[mtx][t][2 * h] * d0, acc[mtx][t][2 * h + 1] * d1);
               }
         clear();
-        __syncthreads();
-        for (int o = threadIdx.x; o < 16 * M; o += blockDim.x) {
-          const int row = o % 16, m = o / 16, n = tile * 16 + row;
-          float v[NM];
+        if (++done % meet == 0 || done == mine_tiles) {
+          const int first = (done - 1) / meet * meet;
+          __syncthreads();
+          for (int o = threadIdx.x; o < (done - first) * 16 * M; o += blockDim.x) {
+            const int row = o % 16, m = MT == 1 ? o / 16 % M : o / 16, tl = MT == 1 ? o / (16 * M) : 0;
+            const int n = ((int)blockIdx.x + (first + tl) * (int)gridDim.x) * 16 + row;
+            const float* src = red + tl * red_n + row * rp + m;
+            float v[NM];
 #pragma unroll
-          for (int mtx = 0; mtx < NM; ++mtx) {
-            v[mtx] = 0.f;
-            for (int w = 0; w < nw; ++w) v[mtx] += red[((mtx * nw + w) * 16 + row) * rp + m];
+            for (int mtx = 0; mtx < NM; ++mtx) {
+              v[mtx] = 0.f;
+#pragma unroll 4
+              for (int w = 0; w < nw; ++w) v[mtx] += src[(mtx * nw + w) * 16 * rp];
+            }
+            if (n < N) static_cast<T*>(p.y)[(int64_t)m * p.ldy + n] = from_f<T>(GATE ? silu_mul(v[0], v[NM - 1]) : v[0]);
           }
-          if (n < N) static_cast<T*>(p.y)[(int64_t)m * p.ldy + n] = from_f<T>(GATE ? silu_mul(v[0], v[NM - 1]) : v[0]);
+          if (done < mine_tiles) __syncthreads();  // (before the next tiles' sums)
         }
-        tile += gridDim.x;
       }
     }
   }
@@ -692,7 +701,7 @@ size_t smem_bytes(int MT, bool gate, int kslice) {
   return (size_t)MP * (kslice + 32) * 2 + (size_t)(gate ? 2 : 1) * kRows * (MP + 2) * sizeof(float);
 }
 constexpr size_t kMaxSmem = 220 * 1024;
-constexpr size_t kStreamSmem = 226 * 1024;
+constexpr size_t kStreamSmem = 227 * 1024;
 
 int kslice_of(int K, int cs) {
   const int per = (K + cs - 1) / cs;
@@ -705,14 +714,14 @@ int stream_warps(int K) {
   return (nsl + rounds - 1) / rounds;
 }
 bool stream_xreg(int K) { return (K + kSlice - 1) / kSlice <= kStreamWarps; }
-size_t stream_smem(int M, int K, bool gate) {
+size_t stream_smem(int M, int K, bool gate, int meet) {
   const int nm = gate ? 2 : 1, nw = stream_warps(K), nsl = (K + kSlice - 1) / kSlice;
   const bool xreg = stream_xreg(K);
-  return (size_t)nw * stream_depth(gate, xreg) * nm * 2048 + sizeof(float) * nm * nw * 16 * ((M + 1) & ~1) +
+  return (size_t)nw * stream_depth(gate, xreg) * nm * 2048 + (size_t)meet * sizeof(float) * nm * nw * 16 * ((M + 1) & ~1) +
          (xreg ? 0 : (size_t)M * (nsl * kSlice + 32) * 2 + (size_t)nsl * 8 * sizeof(float));
 }
 bool stream_fits(int M, int K, bool gate) {
-  return M <= 16 && (M <= 8 || stream_xreg(K)) && stream_smem(M, K, gate) <= kStreamSmem;
+  return M <= 16 && (M <= 8 || stream_xreg(K)) && stream_smem(M, K, gate, 1) <= kStreamSmem;
 }
 
 template <typename T, int MT, int G, bool GATE, bool XREG>
@@ -726,9 +735,13 @@ int launch_stream(const W4Params& p, cudaStream_t st) {
       return B200MM_ERR_LAUNCH;
     configured[dev] = true;
   }
-  const int tiles = (p.N + 15) / 16, sms = num_sms(dev);
-  return launch_pdl(kern, dim3(tiles < sms ? tiles : sms), dim3(32 * stream_warps(p.K)), stream_smem(p.M, p.K, GATE), st,
-                    p) == cudaSuccess
+  const int tiles = (p.N + 15) / 16, sms = num_sms(dev), grid = tiles < sms ? tiles : sms;
+  // the warps meet as rarely as shared memory allows (measured, one row: a meeting per tile costs the
+  // gate-up call 4 of its 17 us)
+  int meet = MT == 1 ? (tiles + grid - 1) / grid : 1;
+  while (meet > 1 && stream_smem(p.M, p.K, GATE, meet) > kStreamSmem) --meet;
+  return launch_pdl(kern, dim3(grid), dim3(32 * stream_warps(p.K)), stream_smem(p.M, p.K, GATE, meet), st, p, meet) ==
+                 cudaSuccess
              ? B200MM_OK
              : B200MM_ERR_LAUNCH;
 }
