@@ -25,8 +25,10 @@
 //     rounded to fp16 (11 bits, and 2^-38 of the block's largest still counts),
 //     the block's O in fp32, joined to the running sums with one factor
 //     that also carries the block's scale of V.
-// Each warp writes one partial (max, sum, O) per (row, head) that its range
-// touches; a second kernel joins them.
+// Each warp has one partial (max, sum, O) per (row, head) that its range touches.
+// Those of a CTA's warps that end in the same pair are joined in shared memory
+// (one long row of 8 KV heads: 18 partials per pair instead of 148, and 15 -> 4
+// us for the second kernel, which joins the rest).
 //
 // Other shapes (fp32, head dims other than 64 / 128, more than 16 query heads
 // per KV head) run a kernel of one CTA per (head, row) on plain arithmetic.
@@ -58,7 +60,8 @@ struct AttnArgs {
 // context); warp i of W (no more than there are units, so that no range is
 // empty) takes [i T / W, (i + 1) T / W).  Partials of warp i for pair
 // p = row KV + head go to slot i + p, distinct for every (i, p) that meet
-// (ranges are contiguous).  Units are whole blocks once every warp has two of
+// (ranges are contiguous); a warp that ends in the pair in which the one before
+// it in its CTA ends has its partial joined to that one's.  Units are whole blocks once every warp has two of
 // them, and 16 tokens below that, so that short contexts spread over the SMs.
 struct Plan {
   int64_t T;
@@ -143,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
   extern __shared__ __align__(1024) unsigned char ring[];
   __shared__ int pre[kMaxRows + 1];     // units of one head in rows before b
   __shared__ long long red[2][kWarps];
+  __shared__ int last_s[kWarps];        // the pair that a warp's range ends in
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
@@ -203,7 +207,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
     __syncthreads();
   }
   const int wi = blockIdx.x * kWarps + warp;
-  if (wi >= plan.W) return;
+  int last_pair = -1;  // none: the warp has no work
+  // state of the running pair
+  uint32_t qf[NH][J][4][2];  // B fragments of q
+  float qinv[NH][2];         // 1 / q's power of two, heads 2c, 2c + 1 (times scale, log2 units)
+  float o[NH][MT][4];
+  float m[NH][2], l[NH][2];  // max and this lane's sum, heads 2c, 2c + 1
+  auto end_pair = [&](float* acc, float* ml) {  // the partial of the pair: [g][D], [g][2]
+#pragma unroll
+    for (int n = 0; n < NH; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float sum = l[n][k];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int h = 8 * n + 2 * c + k;
+        if (h < a.g) {
+          // m-tile i holds d = 2 MT r' + 2i (rows r' = r) and + 1 (rows r + 8)
+          float* dst = acc + h * D + 2 * MT * r;
+#pragma unroll
+          for (int i = 0; i < MT; i += 2)
+            *reinterpret_cast<float4*>(dst + 2 * i) =
+                make_float4(o[n][i][k], o[n][i][2 + k], o[n][i + 1][k], o[n][i + 1][2 + k]);
+          if (r == 0) *reinterpret_cast<float2*>(ml + h * 2) = make_float2(m[n][k], sum);
+        }
+      }
+  };
+
+  if (wi < plan.W) {
   const int64_t u0 = (int64_t)wi * plan.T / plan.W, u1 = (int64_t)(wi + 1) * plan.T / plan.W;
 
   // ---- the load cursor: next segment at unit `un` of pair (nb, nh) ----
@@ -265,11 +297,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
     }
   };
 
-  // ---- state of the running pair ----
-  uint32_t qf[NH][J][4][2];  // B fragments of q
-  float qinv[NH][2];         // 1 / q's power of two, heads 2c, 2c + 1 (times scale, log2 units)
-  float o[NH][MT][4];
-  float m[NH][2], l[NH][2];  // max and this lane's sum, heads 2c, 2c + 1
   auto begin_pair = [&](const Seg& s) {
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
@@ -317,29 +344,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
       l[n][0] = l[n][1] = 0.f;
     }
   };
-  auto end_pair = [&](int b, int kvh) {
-    const int64_t slot = (int64_t)wi + (int64_t)b * KV + kvh;
-#pragma unroll
-    for (int n = 0; n < NH; ++n)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float sum = l[n][k];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        const int h = 8 * n + 2 * c + k;
-        if (h < a.g) {
-          // m-tile i holds d = 2 MT r' + 2i (rows r' = r) and + 1 (rows r + 8)
-          float* dst = a.pacc + (slot * a.g + h) * D + 2 * MT * r;
-#pragma unroll
-          for (int i = 0; i < MT; i += 2)
-            *reinterpret_cast<float4*>(dst + 2 * i) =
-                make_float4(o[n][i][k], o[n][i][2 + k], o[n][i + 1][k], o[n][i + 1][2 + k]);
-          if (r == 0) *reinterpret_cast<float2*>(a.pml + (slot * a.g + h) * 2) = make_float2(m[n][k], sum);
-        }
-      }
-  };
-
   Seg cur, nxt;
   bool more = next_seg(cur);  // a range is not empty
   int slot = 0;               // of cur's K; its V is in the next one
@@ -484,18 +488,46 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
           for (int e = 0; e < 4; ++e) o[n][i][e] = o[n][i][e] * fo[n][e & 1] + ob[n][i][e] * fb[n][e & 1];
     }
     __syncwarp();
-    if (!more) {
-      end_pair(cur.b, cur.kvh);
-      break;
-    }
+    if (!more) break;
     if (nxt.b != cur.b || nxt.kvh != cur.kvh) {
-      end_pair(cur.b, cur.kvh);
+      const int64_t at = ((int64_t)wi + (int64_t)cur.b * KV + cur.kvh) * a.g;
+      end_pair(a.pacc + at * D, a.pml + at * 2);
       begin_pair(nxt);
     }
     cur = nxt;
     slot = slot_n;
   }
   cp_wait<0>();
+  last_pair = cur.b * KV + cur.kvh;
+  }  // (warps with work)
+
+  // ---- the last partials of the CTA's warps, joined where they are of one pair ----
+  __syncthreads();  // the rings are empty
+  float* sacc = reinterpret_cast<float*>(ring);          // [warp][g][D]
+  float* sml = sacc + (size_t)kWarps * a.g * D;          // [warp][g][2]
+  if (last_pair >= 0) end_pair(sacc + (size_t)warp * a.g * D, sml + warp * a.g * 2);
+  if (lane == 0) last_s[warp] = last_pair;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kWarps * a.g * (D / 4); i += kThreads) {
+    const int d = i % (D / 4) * 4, h = i / (D / 4) % a.g, w0 = i / (D / 4) / a.g;
+    const int pair = last_s[w0];
+    if (pair < 0 || (w0 > 0 && last_s[w0 - 1] == pair)) continue;  // no work, or joined to the one before
+    int w1 = w0 + 1;
+    float mx = sml[(w0 * a.g + h) * 2];
+    for (; w1 < kWarps && last_s[w1] == pair; ++w1) mx = fmaxf(mx, sml[(w1 * a.g + h) * 2]);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    for (int q = w0; q < w1; ++q) {
+      const float2 ml = *reinterpret_cast<const float2*>(sml + (q * a.g + h) * 2);
+      const float f = ml.x == mx ? 1.f : ex2(ml.x - mx);
+      const float4 o4 = *reinterpret_cast<const float4*>(sacc + ((size_t)q * a.g + h) * D + d);
+      v.x = fmaf(o4.x, f, v.x); v.y = fmaf(o4.y, f, v.y); v.z = fmaf(o4.z, f, v.z); v.w = fmaf(o4.w, f, v.w);
+      l = fmaf(ml.y, f, l);
+    }
+    const int64_t at = ((int64_t)blockIdx.x * kWarps + w0 + pair) * a.g + h;
+    *reinterpret_cast<float4*>(a.pacc + at * D + d) = v;
+    if (d == 0) *reinterpret_cast<float2*>(a.pml + at * 2) = make_float2(mx, l);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -548,8 +580,14 @@ __global__ void __launch_bounds__(kThreads) kv8_join_kernel(const __grid_constan
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool mine = 4 * lane < D;
+  // partials: warp i0's, the first of each later CTA, and warp i1's if it goes on to the next pair
+  // (otherwise it ends here, as all between do, and is joined to its CTA's)
+  const int first = (i0 / kWarps + 1) * kWarps;
+  const int later = i1 < first ? 0 : (i1 - first) / kWarps + 1;
+  const bool own = i1 > i0 && i1 % kWarps != 0 && (int64_t)(i1 + 1) * plan.T / plan.W > hi;
 #pragma unroll 4
-  for (int i = i0 + warp; i <= i1; i += kWarps) {
+  for (int k = warp; k < 1 + later + (own ? 1 : 0); k += kWarps) {
+    const int i = k == 0 ? i0 : k <= later ? first + (k - 1) * kWarps : i1;
     const int64_t slot = (i + p) * a.g + hl;
     const float2 ml = *reinterpret_cast<const float2*>(a.pml + slot * 2);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
