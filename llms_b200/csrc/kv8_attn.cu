@@ -38,9 +38,8 @@ namespace b200mm {
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kSlots = 3;       // ring slots per warp
+constexpr int kThreads = 256;   // of the other kernels
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRows = 1024;  // rows of one launch (their lengths are summed by one CTA)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -51,26 +50,37 @@ struct AttnArgs {
   int B, H, g;  // g = H / KV
   Kv8Pos pos;
   float scale;
-  int W;        // warps of the split kernel
+  int W, cw;    // warps of the split kernel, and of a CTA of it
   float* pacc;  // [W + B KV][g][D]: O, relative to the partial's max
   float* pml;   // [W + B KV][g][2]: max (log2 units), sum
 };
 
-// The work of a launch: T units of `ut` tokens, flattened over (row, KV head,
+// The work of a launch: T units of 2^lg tokens, flattened over (row, KV head,
 // context); warp i of W (no more than there are units, so that no range is
-// empty) takes [i T / W, (i + 1) T / W).  Partials of warp i for pair
-// p = row KV + head go to slot i + p, distinct for every (i, p) that meet
-// (ranges are contiguous); a warp that ends in the pair in which the one before
-// it in its CTA ends has its partial joined to that one's.  Units are whole blocks once every warp has two of
-// them, and 16 tokens below that, so that short contexts spread over the SMs.
+// empty) takes T / W of them, the first T mod W warps one more.  Partials of
+// warp i for pair p = row KV + head go to slot i + p, distinct for every (i, p)
+// that meet (ranges are contiguous); a warp that ends in the pair in which the
+// one before it in its CTA ends has its partial joined to that one's.  Units are
+// whole blocks where every warp has many, and 16 tokens below that, so that
+// short contexts spread over the SMs and the ranges are even.
+// (T fits 32 bits: 2^31 blocks would be 2 TB of cache.)
 struct Plan {
-  int64_t T;
-  int ut, W;
+  int T, lg, W, per, more;  // per = T / W, more = T mod W
+  __device__ __forceinline__ int begin(int i) const { return i * per + min(i, more); }
+  __device__ __forceinline__ int warp_of(int u) const {
+    const int cut = more * (per + 1);
+    return u < cut ? u / (per + 1) : more + (u - cut) / per;
+  }
 };
-__device__ __forceinline__ int units(int len, int ut) { return (len + ut - 1) / ut; }
+__device__ __forceinline__ int units(int len, int lg) { return (len + (1 << lg) - 1) >> lg; }
 __device__ __forceinline__ Plan make_plan(int64_t n64, int64_t n16, int W) {
-  if (n64 >= 2 * (int64_t)W) return Plan{n64, 64, W};
-  return Plan{n16, 16, n16 < W ? (int)n16 : W};
+  Plan p;
+  p.lg = n64 >= 8 * (int64_t)W ? 6 : 4;
+  p.T = (int)(p.lg == 6 ? n64 : n16);
+  p.W = p.T < W ? p.T : W;
+  p.per = p.W ? p.T / p.W : 0;
+  p.more = p.T - p.per * p.W;
+  return p;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -136,15 +146,21 @@ struct Seg {
   float sk, sv;
 };
 
+// Warps per CTA: as many as the registers allow.  With eight the kernel waited
+// for its own instructions two thirds of the time (two warps per scheduler).
+__host__ __device__ constexpr int split_warps(int NH) { return NH == 1 ? 12 : 8; }
+
 template <typename T, int D, int NH>
-__global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int kWarps = split_warps(NH), kThreads = 32 * kWarps;
   constexpr int J = D / 64;             // 16-byte chunks of a K row per lane
   constexpr int MT = D / 16;            // m-tiles of O^T
   constexpr uint32_t SLOT = 64 * D;     // bytes
   constexpr int CPR = D / 16;           // 16-byte chunks per row
   constexpr int RPI = 32 / CPR;         // rows per warp-wide copy
   extern __shared__ __align__(1024) unsigned char ring[];
-  __shared__ int pre[kMaxRows + 1];     // units of one head in rows before b
+  constexpr int PT = (kMaxRows + kThreads - 1) / kThreads;
+  __shared__ int pre[PT * kThreads + 1];  // units of one head in rows before b
   __shared__ long long red[2][kWarps];
   __shared__ int last_s[kWarps];        // the pair that a warp's range ends in
 
@@ -153,19 +169,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
   pdl_trigger();
   pdl_wait();
 
-  // the plan: lengths summed over the rows
+  // the plan: lengths summed over the rows; one position for all rows needs no sum
   const int KV = a.c.KV;
+  const bool even = a.pos.stride == 0;
   Plan plan;
-  {
-    constexpr int PT = kMaxRows / kThreads;
+  int nu0 = 0;  // units of a head, one position for all
+  if (even) {
+    const int len = kv8_len(a.pos(0), a.c.S);
+    plan = make_plan((int64_t)a.B * KV * units(len, 6), (int64_t)a.B * KV * units(len, 4), a.W);
+    nu0 = units(len, plan.lg);
+  } else {
     int len[PT];
     long long n64 = 0, n16 = 0;
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int b = threadIdx.x * PT + i;
       len[i] = b < a.B ? kv8_len(a.pos(b), a.c.S) : 0;
-      n64 += units(len[i], 64);
-      n16 += units(len[i], 16);
+      n64 += units(len[i], 6);
+      n16 += units(len[i], 4);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -187,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
     __syncthreads();
     int mine = 0;
 #pragma unroll
-    for (int i = 0; i < PT; ++i) mine += units(len[i], plan.ut);
+    for (int i = 0; i < PT; ++i) mine += units(len[i], plan.lg);
     int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -201,9 +222,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       pre[threadIdx.x * PT + i] = base;
-      base += units(len[i], plan.ut);
+      base += units(len[i], plan.lg);
     }
-    if (threadIdx.x == kThreads - 1) pre[kMaxRows] = base;
+    if (threadIdx.x == kThreads - 1) pre[PT * kThreads] = base;
     __syncthreads();
   }
   const int wi = blockIdx.x * kWarps + warp;
@@ -236,12 +257,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
   };
 
   if (wi < plan.W) {
-  const int64_t u0 = (int64_t)wi * plan.T / plan.W, u1 = (int64_t)(wi + 1) * plan.T / plan.W;
+  const int u0 = plan.begin(wi);
 
   // ---- the load cursor: next segment at unit `un` of pair (nb, nh) ----
-  int nb, nh, un, nu;
-  int64_t rem = u1 - u0;
-  {
+  int nb, nh, un, nu, len;
+  int rem = plan.begin(wi + 1) - u0;
+  if (even) {
+    const int pair = u0 / nu0;
+    nb = pair / KV;
+    nh = pair - nb * KV;
+    un = u0 - pair * nu0;
+    nu = nu0;
+  } else {
     int lo = 0, hi = a.B - 1;  // the last row with KV pre[row] <= u0 (it is not empty)
     while (lo < hi) {
       const int m = (lo + hi + 1) >> 1;
@@ -249,31 +276,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
     }
     nb = lo;
     nu = pre[nb + 1] - pre[nb];
-    const int64_t v = u0 - (int64_t)pre[nb] * KV;
-    nh = (int)(v / nu);
-    un = (int)(v - (int64_t)nh * nu);
+    const int v = u0 - pre[nb] * KV;
+    nh = v / nu;
+    un = v - nh * nu;
   }
+  len = kv8_len(a.pos(nb), a.c.S);
   auto next_seg = [&](Seg& s) -> bool {
     if (rem <= 0) return false;
     if (un == nu) {  // next pair; rows without tokens have none
       un = 0;
       if (++nh == KV) {
         nh = 0;
-        do { ++nb; } while (pre[nb + 1] == pre[nb]);
-        nu = pre[nb + 1] - pre[nb];
+        ++nb;
+        if (!even) {
+          while (pre[nb + 1] == pre[nb]) ++nb;
+          nu = pre[nb + 1] - pre[nb];
+          len = kv8_len(a.pos(nb), a.c.S);
+        }
       }
     }
-    const int len = kv8_len(a.pos(nb), a.c.S);
-    const int t = un * plan.ut;
+    const int t = un << plan.lg;
     s.b = nb;
     s.kvh = nh;
     s.blk = t >> 6;
     s.valid = min(64, len - (s.blk << 6));
-    int n = plan.ut == 64 ? 1 : 4 - ((t & 63) >> 4);  // units left in this block
-    n = min(n, nu - un);
-    if (n > rem) n = (int)rem;
     s.s0 = (t & 63) >> 4;
-    s.s1 = min(s.s0 + (n * plan.ut >> 4), (s.valid + 15) >> 4);
+    const int n = plan.lg == 6 ? 1 : min(min(4 - s.s0, nu - un), rem);  // units of this block
+    s.s1 = min(s.s0 + (n << (plan.lg - 4)), (s.valid + 15) >> 4);
     un += n;
     rem -= n;
     const int64_t o = (int64_t)s.b * a.c.s_sb + (int64_t)s.kvh * a.c.s_sh + s.blk;
@@ -282,18 +311,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
     return true;
   };
 
-  unsigned char* my = ring + (size_t)warp * kSlots * SLOT;
-  const uint32_t my_u = static_cast<uint32_t>(__cvta_generic_to_shared(my));
-  auto issue = [&](const Seg& s, bool is_v, int slot) {
+  // the warp's two slots: K and V of a block
+  const uint32_t slot_k = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + warp * 2 * SLOT, slot_v = slot_k + SLOT;
+  // a lane's place in a copy of RPI rows; for V it takes turns (rows / 2 mod 4 decides)
+  const uint32_t put_k = slot_k + slot_off<D, false>(lane / CPR, lane % CPR);
+  const uint32_t put_v0 = slot_v + slot_off<D, true>(lane / CPR, lane % CPR);
+  const uint32_t put_v1 = slot_v + slot_off<D, true>(RPI + lane / CPR, lane % CPR) - RPI * D;
+  auto issue = [&](const Seg& s, bool is_v) {
     const int8_t* src = (is_v ? a.c.vq : a.c.kq) + (int64_t)s.b * a.c.q_sb + (int64_t)s.kvh * a.c.q_sh +
                         (int64_t)s.blk * (64 * D) + lane * 16;
-    const uint32_t dst = my_u + slot * SLOT;
+    const bool all = s.s1 - s.s0 == 4;
 #pragma unroll
     for (int i = 0; i < 64 / RPI; ++i) {
-      const int row = i * RPI + lane / CPR, ch = lane % CPR;
       const int st = i * RPI / 16;
-      if (st >= s.s0 && st < s.s1)
-        cp_async16(dst + (is_v ? slot_off<D, true>(row, ch) : slot_off<D, false>(row, ch)), src + i * 512);
+      if (all || (st >= s.s0 && st < s.s1)) cp_async16((is_v ? (i & 1 ? put_v1 : put_v0) : put_k) + i * RPI * D, src + i * 512);
     }
   };
 
@@ -346,36 +377,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
   };
   Seg cur, nxt;
   bool more = next_seg(cur);  // a range is not empty
-  int slot = 0;               // of cur's K; its V is in the next one
-  issue(cur, false, 0);
+  issue(cur, false);
   cp_commit();
-  issue(cur, true, 1);
+  issue(cur, true);
   cp_commit();
   begin_pair(cur);
   while (true) {
     more = next_seg(nxt);
-    const int slot_v = slot + 1 == kSlots ? 0 : slot + 1;
-    const int slot_n = slot_v + 1 == kSlots ? 0 : slot_v + 1;
-    if (more) issue(nxt, false, slot_n);
-    cp_commit();
-    cp_wait<2>();  // cur's K
+    const bool all = cur.s1 - cur.s0 == 4 && cur.valid == 64;  // a whole block
+    cp_wait<1>();  // cur's K
     __syncwarp();
 
     // ---- S = K Q ----
     float sc[NH][4][4];
     {
-      const uint32_t kb = my_u + slot * SLOT;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[n][s][e] = 0.f;
-        if (s >= cur.s0 && s < cur.s1) {
+        if (all || (s >= cur.s0 && s < cur.s1)) {
 #pragma unroll
           for (int j = 0; j < J; ++j) {
-            const uint4 lo = lds16(kb + slot_off<D, false>(16 * s + r, 4 * j + c));
-            const uint4 hi = lds16(kb + slot_off<D, false>(16 * s + r + 8, 4 * j + c));
+            const uint4 lo = lds16(slot_k + slot_off<D, false>(16 * s + r, 4 * j + c));
+            const uint4 hi = lds16(slot_k + slot_off<D, false>(16 * s + r + 8, 4 * j + c));
             const uint32_t L[4] = {lo.x ^ 0x80808080u, lo.y ^ 0x80808080u, lo.z ^ 0x80808080u, lo.w ^ 0x80808080u};
             const uint32_t G[4] = {hi.x ^ 0x80808080u, hi.y ^ 0x80808080u, hi.z ^ 0x80808080u, hi.w ^ 0x80808080u};
 #pragma unroll
@@ -390,35 +416,42 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
       }
     }
     __syncwarp();
-    // cur's K slot is free: nxt's V
-    if (more) issue(nxt, true, slot);
+    if (more) issue(nxt, false);
     cp_commit();
 
     // ---- the block's softmax; tokens outside [16 s0, valid) do not count ----
+    if (!all) {
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (s < cur.s0 || s >= cur.s1 || 16 * s + r + 8 * (e >> 1) >= cur.valid) sc[n][s][e] = -INFINITY;
+    }
     uint32_t pf[NH][4][2];
     float fo[NH][2], fb[NH][2];  // factors of the running and of the block's sums
+    bool same = true;            // no maximum moved
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
-      float mb[2] = {-INFINITY, -INFINITY};
+      float mb[2] = {-INFINITY, -INFINITY}, f[2], ref[2];
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = 16 * s + r + 8 * (e >> 1);
-          const bool on = s >= cur.s0 && s < cur.s1 && t < cur.valid;
-          const float v = on ? sc[n][s][e] * (qinv[n][e & 1] * cur.sk) : -INFINITY;
-          sc[n][s][e] = v;
-          mb[e & 1] = fmaxf(mb[e & 1], v);
-        }
+        for (int e = 0; e < 4; ++e) mb[e & 1] = fmaxf(mb[e & 1], sc[n][s][e]);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         mb[k] = fmaxf(mb[k], __shfl_xor_sync(0xffffffffu, mb[k], 4));
         mb[k] = fmaxf(mb[k], __shfl_xor_sync(0xffffffffu, mb[k], 8));
         mb[k] = fmaxf(mb[k], __shfl_xor_sync(0xffffffffu, mb[k], 16));
-        if (mb[k] == -INFINITY) mb[k] = 0.f;  // no finite score: p is 0 (or NaN where a score is)
+        f[k] = qinv[n][k] * cur.sk;  // (not negative, so it keeps the order)
+        // (a factor that is not finite, or a score: everything below becomes NaN)
+        mb[k] = mb[k] == -INFINITY ? 0.f : __fmul_rn(mb[k], f[k]);
+        ref[k] = 14.f - mb[k];
         const float mn = fmaxf(m[n][k], mb[k]);
         fo[n][k] = ex2(m[n][k] - mn);
         fb[n][k] = ex2(mb[k] - mn);
+        same &= m[n][k] == mn;
         m[n][k] = mn;
       }
       float lb[2] = {0.f, 0.f};
@@ -427,7 +460,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[e] = ex2(sc[n][s][e] - (mb[e & 1] - 14.f));
+          p[e] = ex2(fmaf(sc[n][s][e], f[e & 1], ref[e & 1]));
+          if (!all && sc[n][s][e] == -INFINITY) p[e] = 0.f;  // (a factor of 0 would make it NaN: a block of zero keys)
           lb[e & 1] += p[e];
         }
         pf[n][s][0] = transpose8x8(pack_h2(p[0], p[1]));  // tokens 2c, 2c + 1 of head r
@@ -439,12 +473,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
         fb[n][k] *= cur.sv;
       }
     }
+    same = __all_sync(0xffffffffu, same);
 
-    cp_wait<2>();  // cur's V
+    cp_wait<1>();  // cur's V
     __syncwarp();
     // ---- O = O fo + (V^T P) fb ----
     {
-      const uint32_t vb = my_u + slot_v * SLOT;
       float ob[NH][MT][4];
 #pragma unroll
       for (int n = 0; n < NH; ++n)
@@ -454,15 +488,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
           for (int e = 0; e < 4; ++e) ob[n][i][e] = 0.f;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        if (s >= cur.s0 && s < cur.s1) {
+        if (all || (s >= cur.s0 && s < cur.s1)) {
           const int t = 16 * s + 2 * c;
           uint32_t v0[MT / 2], v1[MT / 2], v8[MT / 2], v9[MT / 2];  // 2 MT bytes of four tokens, from d = 2 MT r
           auto load = [&](uint32_t* dst, int row) {
             if constexpr (D == 128) {
-              const uint4 x = lds16(vb + slot_off<D, true>(row, r));
+              const uint4 x = lds16(slot_v + slot_off<D, true>(row, r));
               dst[0] = x.x; dst[1] = x.y; dst[2] = x.z; dst[3] = x.w;
             } else {
-              const uint2 x = lds8(vb + slot_off<D, true>(row, r >> 1) + 8 * (r & 1));
+              const uint2 x = lds8(slot_v + slot_off<D, true>(row, r >> 1) + 8 * (r & 1));
               dst[0] = x.x; dst[1] = x.y;
             }
           };
@@ -485,9 +519,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][i][e] = o[n][i][e] * fo[n][e & 1] + ob[n][i][e] * fb[n][e & 1];
+          for (int e = 0; e < 4; ++e) {
+            if (!same) o[n][i][e] *= fo[n][e & 1];
+            o[n][i][e] = fmaf(ob[n][i][e], fb[n][e & 1], o[n][i][e]);
+          }
     }
     __syncwarp();
+    if (more) issue(nxt, true);
+    cp_commit();
     if (!more) break;
     if (nxt.b != cur.b || nxt.kvh != cur.kvh) {
       const int64_t at = ((int64_t)wi + (int64_t)cur.b * KV + cur.kvh) * a.g;
@@ -495,7 +534,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
       begin_pair(nxt);
     }
     cur = nxt;
-    slot = slot_n;
   }
   cp_wait<0>();
   last_pair = cur.b * KV + cur.kvh;
@@ -508,25 +546,38 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_split_kernel(const __grid_con
   if (last_pair >= 0) end_pair(sacc + (size_t)warp * a.g * D, sml + warp * a.g * 2);
   if (lane == 0) last_s[warp] = last_pair;
   __syncthreads();
-  for (int i = threadIdx.x; i < kWarps * a.g * (D / 4); i += kThreads) {
-    const int d = i % (D / 4) * 4, h = i / (D / 4) % a.g, w0 = i / (D / 4) / a.g;
-    const int pair = last_s[w0];
-    if (pair < 0 || (w0 > 0 && last_s[w0 - 1] == pair)) continue;  // no work, or joined to the one before
-    int w1 = w0 + 1;
-    float mx = sml[(w0 * a.g + h) * 2];
-    for (; w1 < kWarps && last_s[w1] == pair; ++w1) mx = fmaxf(mx, sml[(w1 * a.g + h) * 2]);
+  // runs of warps that end in one pair: a (run, head) per warp, 4 dims per lane
+  const int theirs = lane < kWarps ? last_s[lane] : -1;
+  const int before = __shfl_up_sync(0xffffffffu, theirs, 1);
+  const unsigned heads = __ballot_sync(0xffffffffu, theirs >= 0 && (lane == 0 || before != theirs));
+  const int runs = __popc(heads) * a.g;
+  for (int i = warp; i < runs; i += kWarps) {
+    const int run = i / a.g, h = i - run * a.g;
+    unsigned rest = heads;
+    for (int k = 0; k < run; ++k) rest &= rest - 1;
+    const int w0 = __ffs(rest) - 1, pair = last_s[w0];
+    rest &= rest - 1;
+    int w1 = rest ? __ffs(rest) - 1 : kWarps;
+    while (last_s[w1 - 1] != pair) --w1;  // (warps without work)
+    // lane = warp: its max and sum
+    const bool in = lane >= w0 && lane < w1;
+    const float2 ml = in ? *reinterpret_cast<const float2*>(sml + (lane * a.g + h) * 2) : make_float2(-INFINITY, 0.f);
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float f = in ? ex2(ml.x - mx) : 0.f;
+    const float sum = warp_sum(in ? ml.y * f : 0.f);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
     for (int q = w0; q < w1; ++q) {
-      const float2 ml = *reinterpret_cast<const float2*>(sml + (q * a.g + h) * 2);
-      const float f = ml.x == mx ? 1.f : ex2(ml.x - mx);
-      const float4 o4 = *reinterpret_cast<const float4*>(sacc + ((size_t)q * a.g + h) * D + d);
-      v.x = fmaf(o4.x, f, v.x); v.y = fmaf(o4.y, f, v.y); v.z = fmaf(o4.z, f, v.z); v.w = fmaf(o4.w, f, v.w);
-      l = fmaf(ml.y, f, l);
+      const float fq = __shfl_sync(0xffffffffu, f, q);
+      if (4 * lane < D) {
+        const float4 o4 = *reinterpret_cast<const float4*>(sacc + ((size_t)q * a.g + h) * D + 4 * lane);
+        v.x = fmaf(o4.x, fq, v.x); v.y = fmaf(o4.y, fq, v.y); v.z = fmaf(o4.z, fq, v.z); v.w = fmaf(o4.w, fq, v.w);
+      }
     }
     const int64_t at = ((int64_t)blockIdx.x * kWarps + w0 + pair) * a.g + h;
-    *reinterpret_cast<float4*>(a.pacc + at * D + d) = v;
-    if (d == 0) *reinterpret_cast<float2*>(a.pml + at * 2) = make_float2(mx, l);
+    if (4 * lane < D) *reinterpret_cast<float4*>(a.pacc + at * D + 4 * lane) = v;
+    if (lane == 0) *reinterpret_cast<float2*>(a.pml + at * 2) = make_float2(mx, sum);
   }
 }
 
@@ -543,51 +594,61 @@ __global__ void __launch_bounds__(kThreads) kv8_join_kernel(const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.c.D, KV = a.c.KV;
   pdl_trigger();
   pdl_wait();
-  long long s[4] = {0, 0, 0, 0};  // units of 64 and of 16 tokens, over all rows and over the rows before b
-  for (int i = threadIdx.x; i < a.B; i += kThreads) {
-    const int len = kv8_len(a.pos(i), a.c.S);
-    s[0] += units(len, 64);
-    s[1] += units(len, 16);
-    if (i < b) {
-      s[2] += units(len, 64);
-      s[3] += units(len, 16);
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
-    if (lane == 0) red[k][warp] = s[k];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    s[k] = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) s[k] += red[k][w];
-  }
   const int len = kv8_len(a.pos(b), a.c.S);
   T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh;
+  long long s[4];  // units of 64 and of 16 tokens, over all rows and over the rows before b
+  if (a.pos.stride == 0) {
+    s[0] = (long long)a.B * units(len, 6);
+    s[1] = (long long)a.B * units(len, 4);
+    s[2] = (long long)b * units(len, 6);
+    s[3] = (long long)b * units(len, 4);
+  } else {
+    s[0] = s[1] = s[2] = s[3] = 0;
+    for (int i = threadIdx.x; i < a.B; i += kThreads) {
+      const int n = kv8_len(a.pos(i), a.c.S), n64 = units(n, 6), n16 = units(n, 4);
+      s[0] += n64;
+      s[1] += n16;
+      if (i < b) {
+        s[2] += n64;
+        s[3] += n16;
+      }
+    }
+    const int busy = min(kWarps, (a.B + 31) / 32);  // warps with rows
+    if (warp < busy) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+        if (lane == 0) red[k][warp] = s[k];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s[k] = 0;
+      for (int w = 0; w < busy; ++w) s[k] += red[k][w];
+    }
+  }
   if (len == 0) {  // a row that is not there
     for (int d = threadIdx.x; d < D; d += kThreads) out[d] = from_f<T>(0.f);
     return;
   }
   const Plan plan = make_plan(s[0] * KV, s[1] * KV, a.W);
-  const int64_t nu = units(len, plan.ut);
-  const int64_t lo = (plan.ut == 64 ? s[2] : s[3]) * KV + kvh * nu, hi = lo + nu;
-  const int i0 = (int)(((lo + 1) * plan.W - 1) / plan.T), i1 = (int)((hi * plan.W - 1) / plan.T);  // lo, hi - 1
+  const int nu = units(len, plan.lg);
+  const int lo = (int)(plan.lg == 6 ? s[2] : s[3]) * KV + kvh * nu, hi = lo + nu;
+  const int i0 = plan.warp_of(lo), i1 = plan.warp_of(hi - 1);
   const int64_t p = (int64_t)b * KV + kvh;
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool mine = 4 * lane < D;
   // partials: warp i0's, the first of each later CTA, and warp i1's if it goes on to the next pair
   // (otherwise it ends here, as all between do, and is joined to its CTA's)
-  const int first = (i0 / kWarps + 1) * kWarps;
-  const int later = i1 < first ? 0 : (i1 - first) / kWarps + 1;
-  const bool own = i1 > i0 && i1 % kWarps != 0 && (int64_t)(i1 + 1) * plan.T / plan.W > hi;
+  const int first = (i0 / a.cw + 1) * a.cw;
+  const int later = i1 < first ? 0 : (i1 - first) / a.cw + 1;
+  const bool own = i1 > i0 && i1 % a.cw != 0 && plan.begin(i1 + 1) > hi;
 #pragma unroll 4
   for (int k = warp; k < 1 + later + (own ? 1 : 0); k += kWarps) {
-    const int i = k == 0 ? i0 : k <= later ? first + (k - 1) * kWarps : i1;
+    const int i = k == 0 ? i0 : k <= later ? first + (k - 1) * a.cw : i1;
     const int64_t slot = (i + p) * a.g + hl;
     const float2 ml = *reinterpret_cast<const float2*>(a.pml + slot * 2);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -686,17 +747,18 @@ bool fast_shape(const b200mm_kv8& c, int H) {
   return c.dtype != B200MM_F32 && (c.D == 64 || c.D == 128) && H / c.KV <= 16;
 }
 
+int cta_warps(const b200mm_kv8& c, int H) { return split_warps(H / c.KV <= 8 ? 1 : 2); }
 // CTAs of the split kernel: one per SM, fewer where the capacity has no work for them
-int split_ctas(const b200mm_kv8& c, int rows) {
+int split_ctas(const b200mm_kv8& c, int rows, int cw) {
   const int64_t most = (int64_t)rows * c.KV * ((c.S + 15) / 16);
-  const int64_t need = (most + kWarps - 1) / kWarps;
+  const int64_t need = (most + cw - 1) / cw;
   const int sms = num_sms(current_device());
   return (int)(need < sms ? need : sms);
 }
 
 template <typename T, int D, int NH>
 int launch_split(const AttnArgs& a) {
-  constexpr size_t smem = (size_t)kWarps * kSlots * 64 * D;
+  constexpr size_t smem = (size_t)split_warps(NH) * 2 * 64 * D;
   auto kern = kv8_split_kernel<T, D, NH>;
   const int dev = current_device();
   static bool configured[64] = {false};
@@ -713,8 +775,8 @@ template <typename T, int D, int NH>
 int run_fast(const AttnArgs& a, cudaStream_t st) {
   const int s = launch_split<T, D, NH>(a);
   if (s != B200MM_OK) return s;
-  constexpr size_t smem = (size_t)kWarps * kSlots * 64 * D;
-  cudaError_t e = launch_pdl(kv8_split_kernel<T, D, NH>, dim3(a.W / kWarps), dim3(kThreads), smem, st, a);
+  constexpr size_t smem = (size_t)split_warps(NH) * 2 * 64 * D;
+  cudaError_t e = launch_pdl(kv8_split_kernel<T, D, NH>, dim3(a.W / a.cw), dim3(32 * a.cw), smem, st, a);
   if (e != cudaSuccess) return B200MM_ERR_LAUNCH;
   e = launch_pdl(kv8_join_kernel<T>, dim3(a.H, a.B), dim3(kThreads), 0, st, a);
   return e == cudaSuccess ? B200MM_OK : B200MM_ERR_LAUNCH;
@@ -738,7 +800,8 @@ int run(const AttnArgs& a, bool fast, cudaStream_t st) {
 size_t kv8_decode_workspace_bytes(const b200mm_kv8& c, int B, int H) {
   if (!fast_shape(c, H)) return 0;
   const int rows = B < kMaxRows ? B : kMaxRows;
-  const size_t slots = (size_t)split_ctas(c, rows) * kWarps + (size_t)rows * c.KV;
+  const int cw = cta_warps(c, H);
+  const size_t slots = (size_t)split_ctas(c, rows, cw) * cw + (size_t)rows * c.KV;
   return slots * (H / c.KV) * (c.D + 2) * sizeof(float);
 }
 
@@ -763,7 +826,8 @@ int kv8_decode(const b200mm_kv8& c, const void* q, int64_t q_sb, int64_t q_sh, v
     if (pos.dev) a.pos.dev += (int64_t)b0 * pos.stride;
     a.scale = scale;
     if (fast) {
-      a.W = split_ctas(c, a.B) * kWarps;
+      a.cw = cta_warps(c, H);
+      a.W = split_ctas(c, a.B, a.cw) * a.cw;
       const int64_t slots = (int64_t)a.W + (int64_t)a.B * c.KV;
       a.pacc = static_cast<float*>(ws);
       a.pml = a.pacc + slots * a.g * c.D;

@@ -267,10 +267,10 @@ def test_more_rows_than_one_launch_takes():
     _check_attn(got, q, kv, lens, 0.125)
 
 
-@pytest.mark.parametrize("spread", ["q large", "q small", "keys", "values", "one hot"])
+@pytest.mark.parametrize("spread", ["q large", "q small", "keys", "values", "one hot", "zero keys", "zero values", "zero q"])
 def test_scales_far_apart(spread):
     """Queries near the ends of bf16's range, blocks whose scales differ by
-    2^40, one token that takes all."""
+    2^40, one token that takes all, zero blocks (the last one of them cut)."""
     from llms_b200.kernels import int8_kv_append, int8_kv_decode_attn
     B, KV, L, D = 1, 2, 400, 128
     k, v = _tokens(B, KV, L, D, seed=6)
@@ -285,6 +285,12 @@ def test_scales_far_apart(spread):
     elif spread == "values":
         v[:, :, 64:128] *= 2.0 ** 20
         v[:, :, 128:192] *= 2.0 ** -20
+    elif spread == "zero keys":
+        k[:, :, 64:128], k[:, :, 384:] = 0, 0
+    elif spread == "zero values":
+        v[:, :, 64:128], v[:, :, 384:] = 0, 0
+    elif spread == "zero q":
+        q[:, 1::2] = 0
     else:
         k[:, :, 200] = q[:, ::4, 0].to(BF) * 4
     q = q.to(BF)
