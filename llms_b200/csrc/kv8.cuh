@@ -21,9 +21,12 @@ __device__ __forceinline__ int kv8_len(int64_t p, int64_t S) { return p < 0 ? 0 
 
 // int8 bytes i of two words -> fp16x2 (exact): the bytes, sign-flipped, become
 // the low mantissa bits of 1024 + (q + 128), and subtracting 1152 leaves q.
-__device__ __forceinline__ uint32_t i8_pair_to_h2(uint32_t w0, uint32_t w1, int i) {
+// `mask` is 0x00ff00ff and `bits` 0x64806480, in registers: one logic
+// instruction takes one literal.
+__device__ __forceinline__ uint32_t i8_pair_to_h2(uint32_t w0, uint32_t w1, int i, uint32_t mask, uint32_t bits) {
   const uint32_t x = __byte_perm(w0, w1, (uint32_t)(0x4400 + 0x1111 * i));
-  const uint32_t h = (x & 0x00ff00ffu) ^ 0x64806480u;
+  uint32_t h;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(h) : "r"(x), "r"(mask), "r"(bits));  // (x & mask) ^ bits
   const __half2 v =
       __hsub2(*reinterpret_cast<const __half2*>(&h), __half2(__float2half(1152.f), __float2half(1152.f)));
   return *reinterpret_cast<const uint32_t*>(&v);

@@ -38,7 +38,7 @@ namespace b200mm {
 
 namespace {
 
-constexpr int kThreads = 256;   // of the other kernels
+constexpr int kThreads = 256;   // of the plain kernel
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRows = 1024;  // rows of one launch (their lengths are summed by one CTA)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -166,6 +166,8 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
+  const uint32_t none = (uint32_t)a.B >> 31;  // 0, unknown to the compiler
+  const uint32_t mask = 0x00ff00ffu + none, bits = 0x64806480u + none;
   pdl_trigger();
   pdl_wait();
 
@@ -507,8 +509,8 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             const int w = i >> 1, k = 2 * (i & 1);
-            const uint32_t a0 = i8_pair_to_h2(v0[w], v1[w], k), a1 = i8_pair_to_h2(v0[w], v1[w], k + 1);
-            const uint32_t a2 = i8_pair_to_h2(v8[w], v9[w], k), a3 = i8_pair_to_h2(v8[w], v9[w], k + 1);
+            const uint32_t a0 = i8_pair_to_h2(v0[w], v1[w], k, mask, bits), a1 = i8_pair_to_h2(v0[w], v1[w], k + 1, mask, bits);
+            const uint32_t a2 = i8_pair_to_h2(v8[w], v9[w], k, mask, bits), a3 = i8_pair_to_h2(v8[w], v9[w], k + 1, mask, bits);
 #pragma unroll
             for (int n = 0; n < NH; ++n) mma_h(ob[n][i], a0, a1, a2, a3, pf[n][s][0], pf[n][s][1]);
           }
@@ -583,19 +585,27 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
 
 // ---------------------------------------------------------------------------
 // join: out[b, h] = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k over the
-// partials of the pair.  grid (H, B), 8 warps over the partials, lane = 4 dims.
+// partials of the pair.  A warp per head, lane = 4 dims; a few partials each, so
+// no more threads, and nothing to wait for among them.
 // ---------------------------------------------------------------------------
+constexpr int kJoinWarps = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) kv8_join_kernel(const __grid_constant__ AttnArgs a) {
-  __shared__ float acc_s[kWarps][128];
-  __shared__ float m_s[kWarps], l_s[kWarps];
-  __shared__ long long red[4][kWarps];
-  const int h = blockIdx.x, b = blockIdx.y, kvh = h / a.g, hl = h % a.g;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.c.D, KV = a.c.KV;
+__global__ void __launch_bounds__(32 * kJoinWarps) kv8_join_kernel(const __grid_constant__ AttnArgs a) {
+  const int lane = threadIdx.x & 31, D = a.c.D, KV = a.c.KV;
+  const int b = blockIdx.y, h = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
   pdl_trigger();
   pdl_wait();
+  if (h >= a.H) return;
+  const int kvh = h / a.g, hl = h - kvh * a.g;
   const int len = kv8_len(a.pos(b), a.c.S);
-  T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh;
+  T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + 4 * lane;
+  const bool mine = 4 * lane < D;
+  if (len == 0) {  // a row that is not there
+    if (mine)
+      for (int e = 0; e < 4; ++e) out[e] = from_f<T>(0.f);
+    return;
+  }
   long long s[4];  // units of 64 and of 16 tokens, over all rows and over the rows before b
   if (a.pos.stride == 0) {
     s[0] = (long long)a.B * units(len, 6);
@@ -604,7 +614,7 @@ __global__ void __launch_bounds__(kThreads) kv8_join_kernel(const __grid_constan
     s[3] = (long long)b * units(len, 4);
   } else {
     s[0] = s[1] = s[2] = s[3] = 0;
-    for (int i = threadIdx.x; i < a.B; i += kThreads) {
+    for (int i = lane; i < a.B; i += 32) {
       const int n = kv8_len(a.pos(i), a.c.S), n64 = units(n, 6), n16 = units(n, 4);
       s[0] += n64;
       s[1] += n16;
@@ -613,72 +623,60 @@ __global__ void __launch_bounds__(kThreads) kv8_join_kernel(const __grid_constan
         s[3] += n16;
       }
     }
-    const int busy = min(kWarps, (a.B + 31) / 32);  // warps with rows
-    if (warp < busy) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
-        if (lane == 0) red[k][warp] = s[k];
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      s[k] = 0;
-      for (int w = 0; w < busy; ++w) s[k] += red[k][w];
-    }
-  }
-  if (len == 0) {  // a row that is not there
-    for (int d = threadIdx.x; d < D; d += kThreads) out[d] = from_f<T>(0.f);
-    return;
+      for (int o = 16; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
   }
   const Plan plan = make_plan(s[0] * KV, s[1] * KV, a.W);
   const int nu = units(len, plan.lg);
   const int lo = (int)(plan.lg == 6 ? s[2] : s[3]) * KV + kvh * nu, hi = lo + nu;
   const int i0 = plan.warp_of(lo), i1 = plan.warp_of(hi - 1);
   const int64_t p = (int64_t)b * KV + kvh;
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const bool mine = 4 * lane < D;
   // partials: warp i0's, the first of each later CTA, and warp i1's if it goes on to the next pair
   // (otherwise it ends here, as all between do, and is joined to its CTA's)
   const int first = (i0 / a.cw + 1) * a.cw;
   const int later = i1 < first ? 0 : (i1 - first) / a.cw + 1;
   const bool own = i1 > i0 && i1 % a.cw != 0 && plan.begin(i1 + 1) > hi;
-#pragma unroll 4
-  for (int k = warp; k < 1 + later + (own ? 1 : 0); k += kWarps) {
-    const int i = k == 0 ? i0 : k <= later ? first + (k - 1) * a.cw : i1;
-    const int64_t slot = (i + p) * a.g + hl;
-    const float2 ml = *reinterpret_cast<const float2*>(a.pml + slot * 2);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (mine) v = *reinterpret_cast<const float4*>(a.pacc + slot * D + 4 * lane);
-    const float mn = fmaxf(m, ml.x), f0 = m == mn ? 1.f : ex2(m - mn), f1 = ml.x == mn ? 1.f : ex2(ml.x - mn);
-    acc.x = acc.x * f0 + v.x * f1;
-    acc.y = acc.y * f0 + v.y * f1;
-    acc.z = acc.z * f0 + v.z * f1;
-    acc.w = acc.w * f0 + v.w * f1;
-    l = l * f0 + ml.y * f1;
-    m = mn;
-  }
-  if (lane == 0) {
-    m_s[warp] = m;
-    l_s[warp] = l;
-  }
-  if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float mm = m_s[0];
+  const int n = 1 + later + (own ? 1 : 0);
+  // slot of partial k, from the pair's first: warps apart
+  const int64_t slot0 = (i0 + p) * a.g + hl;
+  auto off_of = [&](int k) { return (k == 0 ? 0 : k <= later ? first + (k - 1) * a.cw - i0 : i1 - i0) * a.g; };
+  const float* pml = a.pml + slot0 * 2;
+  const float* pacc = a.pacc + slot0 * D + 4 * lane;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int U = 16;  // partials at a time: their loads go out together
+  for (int k0 = 0; k0 < n; k0 += U) {
+    const float2 ml = lane < U && k0 + lane < n ? *reinterpret_cast<const float2*>(pml + off_of(k0 + lane) * 2)
+                                                : make_float2(-INFINITY, 0.f);
+    float4 v[U];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) mm = fmaxf(mm, m_s[w]);
-    float num = 0.f, den = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = m_s[w] == -INFINITY ? 0.f : ex2(m_s[w] - mm);
-      num += acc_s[w][threadIdx.x] * f;
-      den += l_s[w] * f;
+    for (int k = 0; k < U; ++k) {
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (mine && k0 + k < n) v[k] = *reinterpret_cast<const float4*>(pacc + off_of(k0 + k) * D);
     }
-    out[threadIdx.x] = from_f<T>(num / den);
+    float mn = ml.x;
+#pragma unroll
+    for (int o = U / 2; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mn = fmaxf(__shfl_sync(0xffffffffu, mn, 0), m);
+    const float f0 = ex2(m - mn), f = ex2(ml.x - mn);
+    m = mn;
+    l = l * f0 + warp_sum(ml.y * f);
+    acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      acc.x = fmaf(v[k].x, fk, acc.x); acc.y = fmaf(v[k].y, fk, acc.y);
+      acc.z = fmaf(v[k].z, fk, acc.z); acc.w = fmaf(v[k].w, fk, acc.w);
+    }
+  }
+  if (mine) {
+    const float inv = 1.f / l;
+    out[0] = from_f<T>(acc.x * inv);
+    out[1] = from_f<T>(acc.y * inv);
+    out[2] = from_f<T>(acc.z * inv);
+    out[3] = from_f<T>(acc.w * inv);
   }
 }
 
@@ -778,7 +776,7 @@ int run_fast(const AttnArgs& a, cudaStream_t st) {
   constexpr size_t smem = (size_t)split_warps(NH) * 2 * 64 * D;
   cudaError_t e = launch_pdl(kv8_split_kernel<T, D, NH>, dim3(a.W / a.cw), dim3(32 * a.cw), smem, st, a);
   if (e != cudaSuccess) return B200MM_ERR_LAUNCH;
-  e = launch_pdl(kv8_join_kernel<T>, dim3(a.H, a.B), dim3(kThreads), 0, st, a);
+  e = launch_pdl(kv8_join_kernel<T>, dim3((a.H + kJoinWarps - 1) / kJoinWarps, a.B), dim3(32 * kJoinWarps), 0, st, a);
   return e == cudaSuccess ? B200MM_OK : B200MM_ERR_LAUNCH;
 }
 
