@@ -142,7 +142,7 @@ int b200mm_qkv_w8(const void* x, int64_t ldx,
  *   s : `dtype` [N, K / group], row stride lds
  *   x, y : `dtype` (F16 or BF16); x 16-byte aligned (address and row stride)
  * K is a multiple of group and at most 65536, N at most 2^24.  y = x W^T, fp32 accumulation, no product rounded;
- * the gate/up variant y = silu(x Wg^T) * (x Wu^T).  From M = 192 on the
+ * the gate/up variant y = silu(x Wg^T) * (x Wu^T).  From M = 65 on the
  * weights are first expanded to `dtype` (rounded once) into the workspace:
  * b200mm_w4_workspace_size bytes (0 below that), 256-byte aligned, owned by
  * the stream until the call completes.

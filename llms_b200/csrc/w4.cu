@@ -23,9 +23,10 @@
 // long K, x lies in shared memory) and fills a ring of its own with cp.async,
 // several tiles ahead, so only the sums of a tile meet at a barrier.  Otherwise K is split over a cluster of CTAs with 128 weight rows
 // each, and the sums meet in distributed shared memory.
-// More rows run in chunks of 64, or, from kDenseRows on, the weights
-// are expanded to 16 bits (rounded once: the tcgen05 GEMM's operands are
-// 16-bit) into the caller's workspace and the dense GEMM takes them.
+// From kDenseRows on the weights are expanded to 16 bits (rounded once: the
+// tcgen05 GEMM's operands are 16-bit) into the caller's workspace and the dense
+// GEMM takes them (12288 x 4096 gate and up: 113 us at 128 rows, where two
+// launches of 64 take 166; 83 us at 64 rows, where this would take 127).
 #include "w4.cuh"
 
 #include <type_traits>
@@ -41,7 +42,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 16 * kWarps;  // weight rows per CTA (and matrix)
 constexpr int kChunk = 128;         // columns per warp and step
 constexpr int kMaxRows = 64;        // rows of x per launch
-constexpr int kDenseRows = 192;     // from here on: expand and run the dense GEMM
+constexpr int kDenseRows = 65;      // from here on: expand and run the dense GEMM
 constexpr size_t kFenceBytes = 16;  // of workspace that the memset between the two writes
 
 struct W4Params {
@@ -544,7 +545,7 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const __grid_constant__ W4
     sp[mtx][1] = s + (int64_t)(v_hi ? row_hi : 0) * p.lds + k_begin / G + c * GPC / 4;
   }
   uint4 wv[U][NM][2];
-  float sv[U][NM][2];  // of this lane's group of the chunk
+  uint32_t sv[U][NM][2];  // scale of this lane's group of the chunk, as it is (converting it here would wait for it)
   auto load = [&](int u, int ch) {
     const bool in = ch < nchunks && k_begin + ch * kChunk + 32 * c < k_end;
 #pragma unroll
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const __grid_constant__ W4
         const bool ok = in && (h ? v_hi : v_lo);
         wv[u][mtx][h] = ok ? __ldcs(reinterpret_cast<const uint4*>(wp[mtx][h] + (int64_t)ch * (kChunk / 2)))
                            : make_uint4(0, 0, 0, 0);
-        sv[u][mtx][h] = ok ? to_f<T>(sp[mtx][h][(int64_t)ch * GPC]) : 0.f;
+        sv[u][mtx][h] = ok ? *reinterpret_cast<const unsigned short*>(sp[mtx][h] + (int64_t)ch * GPC) : 0;
       }
   };
 #pragma unroll
@@ -623,8 +624,9 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const __grid_constant__ W4
             }
           }
           // lane quad + (4 / GPC) g holds the group's scales
-          const float s_lo = GPC == 1 ? sv[u][mtx][0] : __shfl_sync(0xffffffffu, sv[u][mtx][0], (lane & 28) + g * (4 / GPC));
-          const float s_hi = GPC == 1 ? sv[u][mtx][1] : __shfl_sync(0xffffffffu, sv[u][mtx][1], (lane & 28) + g * (4 / GPC));
+          const int from = (lane & 28) + g * (4 / GPC);
+          const float s_lo = scale_of<T>(GPC == 1 ? sv[u][mtx][0] : __shfl_sync(0xffffffffu, sv[u][mtx][0], from));
+          const float s_hi = scale_of<T>(GPC == 1 ? sv[u][mtx][1] : __shfl_sync(0xffffffffu, sv[u][mtx][1], from));
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
             acc[mtx][t][0] = fmaf(part[t][0], s_lo, acc[mtx][t][0]);
@@ -703,6 +705,11 @@ size_t smem_bytes(int MT, bool gate, int kslice) {
 constexpr size_t kMaxSmem = 220 * 1024;
 constexpr size_t kStreamSmem = 227 * 1024;
 
+// CTAs that share K: from 17 rows on an eighth of it is too short to hide what
+// comes before and after (12288 x 4096 gate and up, 32 rows: 70 us as 8, 46 as 4, 51
+// as 2); below that few rows leave little else to do (4096 x 12288, 16 rows: 17 us
+// as 8, 31 as 4).
+constexpr int cluster_of(int MT) { return MT >= 4 ? 4 : 8; }
 int kslice_of(int K, int cs) {
   const int per = (K + cs - 1) / cs;
   return (per + kChunk - 1) / kChunk * kChunk;
@@ -774,7 +781,8 @@ int launch_gate(const W4Params& p, bool gate, cudaStream_t st) {
         return gate ? launch_stream<T, 1, G, true, false>(p, st) : launch_stream<T, 1, G, false, false>(p, st);
     }
   }
-  return gate ? launch_w4<T, MT, G, true, 8>(p, st) : launch_w4<T, MT, G, false, 8>(p, st);
+  constexpr int CS = cluster_of(MT);
+  return gate ? launch_w4<T, MT, G, true, CS>(p, st) : launch_w4<T, MT, G, false, CS>(p, st);
 }
 template <typename T, int MT>
 int launch_group(const W4Params& p, int G, bool gate, cudaStream_t st) {
@@ -793,7 +801,7 @@ int launch_rows(const W4Params& p, int G, bool gate, cudaStream_t st) {
 // Rows of x per launch: as many (a power of two from 8, at most 64) as leave room for the K slice in shared memory.
 int rows_per_launch(const W4Args& a) {
   int m = kMaxRows;
-  while (m > 8 && smem_bytes(m / 8, a.gate, kslice_of(a.K, 8)) > kMaxSmem) m /= 2;
+  while (m > 8 && smem_bytes(m / 8, a.gate, kslice_of(a.K, cluster_of(m / 8))) > kMaxSmem) m /= 2;
   return m;
 }
 
@@ -825,7 +833,7 @@ int run_t(const W4Args& a) {
     p.s[0] = a.s0; p.s[1] = a.s1; p.lds = a.lds;
     p.y = static_cast<T*>(a.y) + (int64_t)m0 * a.ldy; p.ldy = a.ldy;
     p.M = a.M - m0 < step ? a.M - m0 : step; p.N = a.N; p.K = a.K;
-    p.kslice = kslice_of(a.K, 8);
+    p.kslice = kslice_of(a.K, cluster_of(p.M <= 8 ? 1 : p.M <= 16 ? 2 : 4));
     const int st = launch_rows<T>(p, a.G, a.gate, a.stream);
     if (st != B200MM_OK) return st;
   }

@@ -1,9 +1,9 @@
 """Projections with 4-bit weights vs their formula in 64 bits.
 
-No product is rounded below 192 rows.  The sums: K / 16 instructions' sums,
+No product is rounded up to 64 rows.  The sums: K / 16 instructions' sums,
 K / group scaled ones, 8 partial ones, each rounded (or cut) within 2^-23 of what
 stands there, at most mass = sum_k |x w|; then half a step of the output's type.
-From 192 rows on each weight is rounded too, half a step of its type."""
+Beyond that each weight is rounded too, half a step of its type."""
 
 import pytest
 import torch
@@ -44,7 +44,7 @@ def _product(x, w, s):
     """(x W^T, its bound) in 64 bits."""
     W, K = _dense(w, s), x.shape[1]
     mass = x.double().abs() @ W.abs().T
-    eps = torch.finfo(x.dtype).eps / 2 if x.shape[0] >= 192 else 0.0
+    eps = torch.finfo(x.dtype).eps / 2 if x.shape[0] > 64 else 0.0
     return x.double() @ W.T, ((K / 16 + s.shape[1] + 8) * 2.0 ** -23 + eps) * mass
 
 
