@@ -69,7 +69,7 @@ class Int8KV:
         self.kq, self.ks, self.kt, self.vq, self.vs, self.vt = kq, ks, kt, vq, vs, vt
         self.rows, self.num_kv_heads, self.capacity, self.head_dim = rows, KV, S, D
         self.dtype, self.device = kt.dtype, kq.device
-        self.length = 0
+        self._length, self._tail = 0, -1
         self._c = _capi.Kv8(kq.data_ptr(), ks.data_ptr(), kt.data_ptr(), vq.data_ptr(), vs.data_ptr(), vt.data_ptr(),
                             kq.stride(0), kq.stride(1), ks.stride(0), ks.stride(1), kt.stride(0), kt.stride(1),
                             S, KV, D, code, 0)
@@ -90,17 +90,26 @@ class Int8KV:
 
         return cls(*half(), *half())
 
+    @property
+    def length(self) -> int:
+        return self._length
+
+    @length.setter
+    def length(self, n: int) -> None:  # by an append that ended at n
+        self._length, self._tail = n, (n - 1) // KV8_BLOCK  # (the block that kt, vt hold)
+
     def rewind(self, n: int) -> None:
         """Forget the tokens from position ``n`` on.  Inside the block that the
         last append ended in the tokens are still there as they came; further
         back the open block's tokens are taken from their 8-bit values."""
-        if not 0 <= n <= self.length:
-            raise ValueError(f"cannot go to position {n}: the cache holds {self.length} tokens")
+        if not 0 <= n <= self._length:
+            raise ValueError(f"cannot go to position {n}: the cache holds {self._length} tokens")
         blk, r = divmod(n, KV8_BLOCK)
-        if r and blk != (self.length - 1) // KV8_BLOCK:
+        if r and blk != self._tail:
             for q, s, t in ((self.kq, self.ks, self.kt), (self.vq, self.vs, self.vt)):
                 t[:, :, :r] = (q[:, :, n - r:n].float() * s[:, :, blk, None, None]).to(t.dtype)
-        self.length = n
+            self._tail = blk
+        self._length = n
 
 
 def _pos(pos, B: int, device: torch.device):
@@ -272,9 +281,13 @@ class Int8KVCache:
 
     @cur_len.setter
     def cur_len(self, n: int) -> None:
-        self._len = n
+        """Up: tokens that a captured step has put in.  Down: :meth:`seek`."""
         for layer in self.layers:
-            layer.length = n
+            if n > layer.length:
+                layer.length = n
+            elif n < layer.length:
+                layer.rewind(n)
+        self._len = n
 
     def seek(self, pos: int) -> None:
         """Make ``pos`` the next position of every layer: where the tokens end,

@@ -357,6 +357,9 @@ class GraphedDecodeStep:
         s.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(s), torch.inference_mode():  # first-call set-up outside the capture
             model.forward_static(self.ids, kv_cache, self.pos)
+            if isinstance(kv_cache, Int8KVCache):  # that token opened its block
+                kv_cache.cur_len += 1
+                kv_cache.seek(kv_cache.cur_len - 1)
         torch.cuda.current_stream(dev).wait_stream(s)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph), torch.inference_mode():
