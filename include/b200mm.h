@@ -228,7 +228,8 @@ int b200mm_gqa_decode(const void* q, int64_t q_sb, int64_t q_sh,
  *            ended in (token t in row t % 64)
  * All zero is the empty cache.  S is a multiple of 64 and at most 2^24; D is a
  * multiple of 16 and at most 256.  kq, vq, kt, vt and their strides are
- * 16-byte aligned.
+ * 16-byte aligned.  Rows and heads do not overlap (one stride covers the other's
+ * blocks).
  *
  * b200mm_kv8_append: tokens k, v [B, KV, T, D] (strides sb, sh, st, unit
  *   inner, 16-byte aligned) enter rows 0..B-1 at positions p .. p + T - 1.  p

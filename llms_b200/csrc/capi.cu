@@ -228,6 +228,7 @@ int run_w4(W4Args& a, int64_t M, int64_t N, int64_t K, int64_t group, size_t ws_
   if (!a.x || !a.w0 || !a.s0 || !a.y || (a.gate && (!a.w1 || !a.s1))) return B200MM_ERR_ARG;
   auto al = [](const void* p) { return ((uintptr_t)p & 15u) == 0; };
   if (!al(a.x) || (a.ldx * 2) % 16 || !al(a.w0) || (a.gate && !al(a.w1)) || a.ldw % 16) return B200MM_ERR_ALIGN;
+  if (((uintptr_t)a.s0 | (uintptr_t)a.s1 | (uintptr_t)a.y) % 2) return B200MM_ERR_ALIGN;
   const size_t need = w4_workspace_bytes(M, N, K, a.gate);
   if (need > 0 && (!a.ws || ws_bytes < need || ((uintptr_t)a.ws & 255u))) return B200MM_ERR_WORKSPACE;
   int st = check_device();
@@ -370,6 +371,13 @@ int b200mm_gqa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* k, 
 namespace {
 bool kv8_al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+// [B, KV] blocks of `n` elements at strides (sb, sh) that do not overlap: heads inside rows, or rows inside heads
+bool kv8_apart(int64_t B, int64_t KV, int64_t sb, int64_t sh, int64_t n) {
+  if (sb < 0 || sh < n) return false;
+  if (B <= 1) return true;
+  return sb >= n && (sb >= (__int128)sh * (KV - 1) + n || sh >= (__int128)sb * (B - 1) + n);
+}
+
 int kv8_check(const b200mm_kv8* c, int64_t B) {
   if (!c) return B200MM_ERR_ARG;
   if (c->dtype != B200MM_F32 && c->dtype != B200MM_F16 && c->dtype != B200MM_BF16) return B200MM_ERR_DTYPE;
@@ -377,19 +385,19 @@ int kv8_check(const b200mm_kv8* c, int64_t B) {
       c->S > (int64_t(1) << 24) || c->S % 64)
     return B200MM_ERR_SHAPE;
   if (!c->kq || !c->ks || !c->kt || !c->vq || !c->vs || !c->vt) return B200MM_ERR_ARG;
-  if (c->q_sh < c->S * c->D || c->q_sb < 0 || c->s_sh < c->S / 64 || c->s_sb < 0 || c->t_sh < 64 * c->D || c->t_sb < 0)
-    return B200MM_ERR_SHAPE;
-  // rows of their own for every batch row
-  if (B > 1 && (c->q_sb < c->S * c->D || c->s_sb < c->S / 64 || c->t_sb < 64 * c->D)) return B200MM_ERR_SHAPE;
   const int esz = c->dtype == B200MM_F32 ? 4 : 2;
   if (!kv8_al16(c->kq) || !kv8_al16(c->vq) || !kv8_al16(c->kt) || !kv8_al16(c->vt) || c->q_sb % 16 || c->q_sh % 16 ||
-      (c->t_sb * esz) % 16 || (c->t_sh * esz) % 16)
+      (c->t_sb * esz) % 16 || (c->t_sh * esz) % 16 || (uintptr_t)c->ks % 4 || (uintptr_t)c->vs % 4)
     return B200MM_ERR_ALIGN;
+  if (!kv8_apart(B, c->KV, c->q_sb, c->q_sh, c->S * c->D) || !kv8_apart(B, c->KV, c->s_sb, c->s_sh, c->S / 64) ||
+      !kv8_apart(B, c->KV, c->t_sb, c->t_sh, 64 * c->D))
+    return B200MM_ERR_SHAPE;
   return B200MM_OK;
 }
 
 int kv8_check_pos(int64_t pos, const int64_t* pos_dev, int64_t pos_stride, int64_t S) {
   if (pos_stride != 0 && pos_stride != 1) return B200MM_ERR_ARG;
+  if ((uintptr_t)pos_dev % 8) return B200MM_ERR_ALIGN;
   if (!pos_dev && (pos < -1 || pos >= S)) return B200MM_ERR_SHAPE;  // a device position is bounded in the kernels
   return B200MM_OK;
 }
@@ -409,7 +417,7 @@ int kv8_check_decode(const b200mm_kv8& c, const void* q, int64_t q_sb, int64_t q
   if (!q || !out || !(scale > 0.f)) return B200MM_ERR_ARG;
   if (q_sb < 0 || q_sh < 0 || o_sb < 0 || o_sh < 0) return B200MM_ERR_SHAPE;
   const int esz = c.dtype == B200MM_F32 ? 4 : 2;
-  if (!kv8_al16(q) || (q_sb * esz) % 16 || (q_sh * esz) % 16) return B200MM_ERR_ALIGN;
+  if (!kv8_al16(q) || (q_sb * esz) % 16 || (q_sh * esz) % 16 || (uintptr_t)out % esz) return B200MM_ERR_ALIGN;
   if (B == 0) return B200MM_OK;
   const size_t need = kv8_decode_workspace_bytes(c, (int)B, (int)H);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255u))) return B200MM_ERR_WORKSPACE;
@@ -494,7 +502,9 @@ int b200mm_token_logprobs(const void* x, int64_t ldx, const int64_t* tokens, flo
   if (top < 0 || top > V || top > kLogprobsMaxTop) return B200MM_ERR_SHAPE;
   if (M == 0) return B200MM_OK;
   if (!x || !tokens || !logprob || !entropy || (top > 0 && (!top_ids || !top_logprobs))) return B200MM_ERR_ARG;
-  if ((uintptr_t)x % (dtype == B200MM_F32 ? 4 : 2)) return B200MM_ERR_ALIGN;
+  if ((uintptr_t)x % (dtype == B200MM_F32 ? 4 : 2) || ((uintptr_t)tokens | (uintptr_t)top_ids) % 8 ||
+      ((uintptr_t)logprob | (uintptr_t)entropy | (uintptr_t)top_logprobs) % 4)
+    return B200MM_ERR_ALIGN;
   int st = check_device();
   if (st != B200MM_OK) return st;
   const LogprobsArgs a{x, ldx, tokens, logprob, entropy, top_ids, top_logprobs, M, (int)V, (int)top};

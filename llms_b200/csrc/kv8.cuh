@@ -1,7 +1,12 @@
 // 8-bit KV cache: layout, bounds and launch entries shared by kv8.cu (append,
 // expand) and kv8_attn.cu (decode attention).
 #pragma once
+#include <cstddef>
+
 #include "common.cuh"
+
+// the layout that the Python mirror of the struct has
+static_assert(sizeof(b200mm_kv8) == 120 && offsetof(b200mm_kv8, S) == 96 && offsetof(b200mm_kv8, KV) == 104);
 
 namespace b200mm {
 
@@ -17,7 +22,7 @@ struct Kv8Pos {
 };
 
 // Tokens that row b attends to, for its last position p: p + 1, at most the capacity; none below 0.
-__device__ __forceinline__ int kv8_len(int64_t p, int64_t S) { return p < 0 ? 0 : (int)(p + 1 < S ? p + 1 : S); }
+__device__ __forceinline__ int kv8_len(int64_t p, int64_t S) { return p < 0 ? 0 : (int)(p < S ? p + 1 : S); }
 
 // int8 bytes i of two words -> fp16x2 (exact): the bytes, sign-flipped, become
 // the low mantissa bits of 1024 + (q + 128), and subtracting 1152 leaves q.

@@ -74,7 +74,7 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
 def _scales(s: torch.Tensor) -> torch.Tensor:
     ld, inner = s.stride()
-    return s if inner == 1 and ld >= s.shape[1] else s.contiguous()
+    return s if inner == 1 and ld >= s.shape[1] else s.clone(memory_format=torch.contiguous_format)
 
 
 def _workspace(x: torch.Tensor, M: int, N: int, K: int, gate: int) -> tuple[torch.Tensor | None, int]:

@@ -52,10 +52,10 @@ def b200_token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int 
         x = x.contiguous()
     M = x.shape[0]
     lead = logits.shape[:-1]
-    lp, ent = x.new_empty((2, *lead), dtype=torch.float32).unbind()
+    lp, ent = x.new_empty(lead, dtype=torch.float32), x.new_empty(lead, dtype=torch.float32)
     ids, lps = x.new_empty((*lead, top), dtype=torch.int64), x.new_empty((*lead, top), dtype=torch.float32)
     if M:
         toks = tokens.contiguous()
-        _capi.launch("b200mm_token_logprobs", x, x.data_ptr(), x.stride(0), toks.data_ptr(), lp.data_ptr(), ent.data_ptr(),
+        _capi.launch("b200mm_token_logprobs", x, x.data_ptr(), x.stride(0) if M > 1 else V, toks.data_ptr(), lp.data_ptr(), ent.data_ptr(),
                      ids.data_ptr(), lps.data_ptr(), M, V, top, code)
     return TokenLogprobs(lp, ent, ids, lps)

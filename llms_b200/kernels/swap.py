@@ -83,6 +83,10 @@ def apply_linear_kernels(model: nn.Module, *, int8: bool = False, o: bool = True
     return model
 
 
+def _dtype_of(lin: nn.Module) -> torch.dtype:
+    return lin.scale.dtype if isinstance(lin, Int4Linear) else lin.weight.dtype
+
+
 def prewarm_triton_kernels(model: nn.Module, *, m_values: tuple[int, ...] = (1, 2, 3, 4, 5, 6, 7, 8)) -> None:
     """Run every swapped projection once per M in ``m_values`` (one module per
     distinct weight shape), so first-call costs (kernel attribute setup,
@@ -113,7 +117,7 @@ def prewarm_triton_kernels(model: nn.Module, *, m_values: tuple[int, ...] = (1, 
             elif isinstance(ffn, Int4FFN):
                 dev, dt = ffn.wg.device, ffn.sg.dtype
             else:
-                dev, dt = ffn.qg.device, ffn.down.weight.dtype
+                dev, dt = ffn.qg.device, _dtype_of(ffn.down)
             for M in m_values:
                 ffn(torch.zeros((1, M, K), dtype=dt, device=dev))
         for key, attn in attns.items():
@@ -123,7 +127,7 @@ def prewarm_triton_kernels(model: nn.Module, *, m_values: tuple[int, ...] = (1, 
                     x = torch.zeros((1, M, K), dtype=attn.s_qkv.dtype, device=attn.w_qkv.device)
                     int4_fused_qkv(x, attn.w_qkv, attn.s_qkv, n_q=attn.n_q, n_k=attn.n_k)
                 elif isinstance(attn, Int8Attention):
-                    x = torch.zeros((1, M, K), dtype=attn.o.weight.dtype, device=attn.q_qkv.device)
+                    x = torch.zeros((1, M, K), dtype=_dtype_of(attn.o), device=attn.q_qkv.device)
                     int8_fused_qkv(x, attn.q_qkv, attn.s_qkv, n_q=attn.n_q, n_k=attn.n_k)
                 else:
                     x = torch.zeros((1, M, K), dtype=attn.W_qkv.dtype, device=attn.W_qkv.device)

@@ -36,6 +36,7 @@ from torch import nn
 
 from . import _capi
 from .kernels.linear import b200_linear, int8_linear
+from .kernels.int4 import Int4Attention, Int4FFN, Int4Linear
 from .kernels.quant import Int8Attention, Int8FFN, int8_fused_gate_up_silu
 
 
@@ -221,6 +222,8 @@ def shard_decode_model(model: nn.Module, rank: int, world: int, group=None, peer
     ``peer`` (a ``peer.PeerGather`` of at least ``peer_bytes(model,
     max_rows)``), the gathers of up to ``max_rows`` tokens run over peer
     memory, one call-site region each.  Returns ``model``."""
+    if any(isinstance(m, (Int4Linear, Int4FFN, Int4Attention)) for m in model.modules()):
+        raise ValueError("projections with 4-bit weights are not sharded")
     dtype = model.layers[0].attn.o.weight.dtype
     for block in model.layers:
         att = ShardedInt8Attention.from_module(block.attn, rank, world, group)

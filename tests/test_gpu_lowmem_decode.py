@@ -195,3 +195,30 @@ def test_prewarm_takes_4_bit_modules():
     from llms_b200.kernels import prewarm_triton_kernels
     m, _ = _models()
     prewarm_triton_kernels(m, m_values=(1, 3))
+
+
+def test_a_step_captured_at_a_border_and_replayed_before_it():
+    """Building the step runs it once, which opens the block at the border;
+    going back into the one before takes that one's tokens up again."""
+    from llms_b200.qwen3 import GraphedDecodeStep
+    m, _ = _models()
+    ids = torch.randint(0, 1000, (2, 80), device="cuda")
+    with torch.inference_mode():
+        c, c2 = (m.alloc_cache(128, max_batch=2, int8=True) for _ in range(2))
+        m(ids[:, :64], c), m(ids[:, :64], c2)  # (the same calls: a product's sums may differ with its rows)
+        m(ids[:, 64:65], c2)
+        step = GraphedDecodeStep(m, c, 2)
+        c2.seek(60)
+        for t in range(60, 70):
+            assert torch.equal(step(ids[:, t:t + 1], t), m(ids[:, t:t + 1], c2))
+        for a, b in zip(c.layers, c2.layers):
+            assert torch.equal(a.kq[:, :, :70], b.kq[:, :, :70]) and torch.equal(a.vs, b.vs)
+
+
+@pytest.mark.parametrize("o,down", [(True, True), (False, True), (True, False)])
+def test_prewarm_takes_8_bit_modules_with_4_bit_outputs(o, down):
+    from llms_b200.kernels import apply_int4_kernels, apply_int8_kernels, prewarm_triton_kernels
+    from llms_b200.qwen3 import QWEN3_4B, Qwen3Model
+    m = Qwen3Model(dataclasses.replace(QWEN3_4B, num_hidden_layers=1, vocab_size=1000)).to("cuda", BF)
+    apply_int4_kernels(apply_int8_kernels(m), o=o, down=down)
+    prewarm_triton_kernels(m, m_values=(1, 3))

@@ -126,3 +126,52 @@ def test_model_cache_counts_and_seeks():
     assert c.cur_len == 64 and [x.length for x in c.layers] == [64, 64]
     with pytest.raises(ValueError):
         c.seek(65)
+
+
+def test_overlapping_rows_or_heads_and_odd_addresses_are_refused():
+    n = 128 * 64
+    for bad, code in (({"q_sb": n, "q_sh": n}, SHAPE), ({"q_sb": 2 * n - 16}, SHAPE), ({"s_sb": 3}, SHAPE),
+                      ({"t_sb": 64 * 64, "t_sh": 64 * 64}, SHAPE), ({"q_sb": n, "q_sh": 2 * n - 16}, SHAPE),
+                      ({"q_sh": 1 << 62, "q_sb": 1 << 62}, SHAPE), ({"ks": 4098}, ALIGN), ({"vs": 4097}, ALIGN)):
+        c = _c_cache(**bad)
+        assert _append(c) == code and _decode(c) == code, bad
+    one_row = _c_cache(q_sb=0, s_sb=0, t_sb=0)
+    assert _append(one_row, B=1, T=0) == OK and _decode(one_row, B=1, ws=None) == WORKSPACE
+    heads_first = _c_cache(q_sb=n, q_sh=2 * n, s_sb=2, s_sh=4, t_sb=64 * 64, t_sh=2 * 64 * 64)
+    assert _append(heads_first, T=0) == OK and _append(heads_first, B=3, T=0) == SHAPE
+    c = _c_cache()
+    assert _capi.lib.b200mm_kv8_append(ctypes.byref(c), 4096, 128, 64, 64, 4096, 128, 64, 64, 2, 1, 0, 4100, 1, None) == ALIGN
+    assert _capi.lib.b200mm_kv8_decode(ctypes.byref(c), 4096, 256, 64, 4097, 256, 64, 2, 4, 0, None, 0, 0.1, 4096, 1 << 30,
+                                       None) == ALIGN
+
+
+def test_struct_layout():
+    """llms_b200._capi.Kv8 has b200mm_kv8's layout (6 pointers, 7 int64, 4 int32)."""
+    off = {n: getattr(_capi.Kv8, n).offset for n, _ in _capi.Kv8._fields_}
+    names = ["kq", "ks", "kt", "vq", "vs", "vt", "q_sb", "q_sh", "s_sb", "s_sh", "t_sb", "t_sh", "S"]
+    assert [off[n] for n in names] == list(range(0, 104, 8))
+    assert [off[n] for n in ("KV", "D", "dtype", "reserved")] == [104, 108, 112, 116] and ctypes.sizeof(_capi.Kv8) == 120
+
+
+def test_going_back_twice_refills_the_open_block():
+    """A token that opened the next block took the place of the first one's
+    tokens: going back to its border, and then further, finds them in 8 bits."""
+    for how in ("rewind", "cur_len"):
+        c = Int8KVCache.alloc(num_layers=1, max_batch=1, num_kv_heads=1, max_seq_len=128, head_dim=64, dtype=torch.float16,
+                              device="cpu")
+        kv = c.layers[0]
+        kv.kq.fill_(3)
+        kv.ks.fill_(0.5)
+        c.cur_len = 65
+        kv.kt.fill_(7)
+        if how == "rewind":
+            c.seek(64)
+            assert (kv.kt == 7).all()
+            c.seek(40)
+        else:
+            c.cur_len = 64
+            c.cur_len = 40
+        assert (kv.kt[0, 0, :40] == 1.5).all() and (kv.kt[0, 0, 40:] == 7).all(), how
+        kv.kt[0, 0, :40] = 9
+        c.seek(10)  # inside the block that is open now
+        assert (kv.kt[0, 0, :40] == 9).all() and c.cur_len == 10 == kv.length

@@ -34,3 +34,10 @@ def test_c_entry_point_refuses_before_any_launch():
     assert call(x=4097) == ALIGN and call(x=4098, dtype=0) == ALIGN
     assert call(M=0) == OK
     assert _capi.launch_count() == before
+
+
+def test_odd_addresses_are_refused():
+    for bad in range(1, 6):
+        p = [4096] * 6
+        p[bad] += 2
+        assert _capi.lib.b200mm_token_logprobs(p[0], 100, *p[1:], 2, 100, 4, 2, None) == 2, bad

@@ -107,3 +107,21 @@ def test_swaps_leave_4_bit_modules_alone():
     m8 = apply_int4_kernels(apply_int8_kernels(Qwen3Model(shape)))
     assert isinstance(m8.layers[0].attn, Int8Attention) and isinstance(m8.layers[0].attn.o, Int4Linear)
     assert m.alloc_cache(40, int8=True).capacity == 64 and m.alloc_cache(40).k[0].shape[2] == 40
+
+
+def test_odd_addresses_are_refused():
+    p = 4096
+    for s, y in ((p + 1, p), (p, p + 1)):
+        assert _capi.lib.b200mm_linear_w4(p, 256, p, 128, s, 2, 128, y, 64, 2, 64, 256, 2, None, 0, None) == 2
+        assert _capi.lib.b200mm_gate_up_silu_w4(p, 256, p, p, 128, p, s, 2, 128, y, 64, 2, 64, 256, 2, None, 0, None) == 2
+
+
+def test_4_bit_models_are_not_sharded():
+    from llms_b200.kernels import apply_int4_kernels, apply_int8_kernels
+    from llms_b200.qwen3 import Qwen3Model, Qwen3Shape
+    from llms_b200.shard import shard_decode_model
+    shape = Qwen3Shape(vocab_size=64, hidden_size=128, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=1,
+                       head_dim=64, intermediate_size=256, max_position_embeddings=32)
+    for m in (apply_int4_kernels(Qwen3Model(shape)), apply_int4_kernels(apply_int8_kernels(Qwen3Model(shape)), o=False)):
+        with pytest.raises(ValueError, match="4-bit"):
+            shard_decode_model(m, 0, 1)
