@@ -437,7 +437,7 @@ int b200mm_kv8_append(const b200mm_kv8* c, const void* k, int64_t k_sb, int64_t 
   if ((st = kv8_check_tokens(*c, v, v_sb, v_sh, v_st)) != B200MM_OK) return st;
   if (B == 0 || T == 0) return B200MM_OK;
   if ((st = check_device()) != B200MM_OK) return st;
-  st = kv8_append(*c, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, (int)B, T, Kv8Pos{pos_dev, pos, (int)pos_stride},
+  st = kv8_append(*c, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, (int)B, T, Kv8Pos{pos_dev, pos, (int)pos_stride}, false,
                   static_cast<cudaStream_t>(stream));
   return st != B200MM_OK ? st : launch_status();
 }
@@ -470,7 +470,7 @@ int b200mm_kv8_decode(const b200mm_kv8* c, const void* q, int64_t q_sb, int64_t 
   if (st != B200MM_OK || B == 0) return st;
   if ((st = check_device()) != B200MM_OK) return st;
   st = kv8_decode(*c, q, q_sb, q_sh, out, o_sb, o_sh, (int)B, (int)H, Kv8Pos{pos_dev, pos, (int)pos_stride}, scale,
-                  workspace, static_cast<cudaStream_t>(stream));
+                  workspace, false, static_cast<cudaStream_t>(stream));
   return st != B200MM_OK ? st : launch_status();
 }
 
@@ -488,9 +488,9 @@ int b200mm_kv8_step(const b200mm_kv8* c, const void* q, int64_t q_sb, int64_t q_
   if ((st = check_device()) != B200MM_OK) return st;
   const Kv8Pos p{pos_dev, pos, (int)pos_stride};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = kv8_append(*c, k, k_sb, k_sh, 0, v, v_sb, v_sh, 0, (int)B, 1, p, s);
+  st = kv8_append(*c, k, k_sb, k_sh, 0, v, v_sb, v_sh, 0, (int)B, 1, p, true, s);
   if (st != B200MM_OK) return st;
-  st = kv8_decode(*c, q, q_sb, q_sh, out, o_sb, o_sh, (int)B, (int)H, p, scale, workspace, s);
+  st = kv8_decode(*c, q, q_sb, q_sh, out, o_sb, o_sh, (int)B, (int)H, p, scale, workspace, true, s);
   return st != B200MM_OK ? st : launch_status();
 }
 

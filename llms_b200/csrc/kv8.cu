@@ -38,6 +38,7 @@ struct AppendArgs {
   int64_t sb[2], sh[2], st[2];
   int64_t T;
   Kv8Pos pos;
+  bool late;  // the next kernel starts when the one before is done (see kv8_decode)
 };
 
 // The largest |x| of a 16-byte chunk and `mx` as bits that order like the values, NaN above
@@ -178,8 +179,9 @@ __device__ void do_block(const T* src, int64_t src_st, T* tail, int8_t* qdst, fl
 template <typename T, int NC>
 __global__ void __launch_bounds__(kThreads, NC == 8 ? 7 : 1) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ uint32_t red[kThreads / 32];
-  pdl_trigger();
+  if (!a.late) pdl_trigger();
   pdl_wait();
+  if (a.late) pdl_trigger();
   // heads next to each other, K before V: together they read whole rows of a projection's output
   const int heads = 2 * a.c.KV, hw = blockIdx.x % heads, which = hw / a.c.KV, h = hw - which * a.c.KV, b = blockIdx.y;
   const int64_t p0 = a.pos(b);
@@ -285,8 +287,8 @@ int expand_t(const ExpandArgs& a, int B, cudaStream_t st) {
 }  // namespace
 
 int kv8_append(const b200mm_kv8& c, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void* v,
-               int64_t v_sb, int64_t v_sh, int64_t v_st, int B, int64_t T, Kv8Pos pos, cudaStream_t st) {
-  const AppendArgs a{c, {k, v}, {k_sb, v_sb}, {k_sh, v_sh}, {k_st, v_st}, T, pos};
+               int64_t v_sb, int64_t v_sh, int64_t v_st, int B, int64_t T, Kv8Pos pos, bool late, cudaStream_t st) {
+  const AppendArgs a{c, {k, v}, {k_sb, v_sb}, {k_sh, v_sh}, {k_st, v_st}, T, pos, late};
   if (c.dtype == B200MM_BF16) return append_t<__nv_bfloat16>(a, B, st);
   if (c.dtype == B200MM_F16) return append_t<__half>(a, B, st);
   return append_t<float>(a, B, st);

@@ -37,12 +37,15 @@ __device__ __forceinline__ uint32_t i8_pair_to_h2(uint32_t w0, uint32_t w1, int 
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// `late`, `early`: a decode step's two halves.  The append lets the attention start as soon as all
+// before the step is done; the attention waits for the append only where it comes to the last block
+// of a row, which is all that the append of one token changes.
 int kv8_append(const b200mm_kv8& c, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void* v,
-               int64_t v_sb, int64_t v_sh, int64_t v_st, int B, int64_t T, Kv8Pos pos, cudaStream_t st);
+               int64_t v_sb, int64_t v_sh, int64_t v_st, int B, int64_t T, Kv8Pos pos, bool late, cudaStream_t st);
 int kv8_expand(const b200mm_kv8& c, void* k, void* v, int64_t o_sb, int64_t o_sh, int64_t o_st, int B, int64_t L,
                cudaStream_t st);
 size_t kv8_decode_workspace_bytes(const b200mm_kv8& c, int B, int H);
 int kv8_decode(const b200mm_kv8& c, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-               int B, int H, Kv8Pos pos, float scale, void* ws, cudaStream_t st);
+               int B, int H, Kv8Pos pos, float scale, void* ws, bool early, cudaStream_t st);
 
 }  // namespace b200mm

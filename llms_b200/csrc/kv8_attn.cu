@@ -50,6 +50,7 @@ struct AttnArgs {
   int B, H, g;  // g = H / KV
   Kv8Pos pos;
   float scale;
+  bool early;   // right behind the append of one token: only the rows' last blocks wait for it
   int W, cw;    // warps of the split kernel, and of a CTA of it
   float* pacc;  // [W + B KV][g][D]: O, relative to the partial's max
   float* pml;   // [W + B KV][g][2]: max (log2 units), sum
@@ -169,7 +170,8 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
   const uint32_t none = (uint32_t)a.B >> 31;  // 0, unknown to the compiler
   const uint32_t mask = 0x00ff00ffu + none, bits = 0x64806480u + none;
   pdl_trigger();
-  pdl_wait();
+  bool waited = !a.early;
+  if (waited) pdl_wait();
 
   // the plan: lengths summed over the rows; one position for all rows needs no sum
   const int KV = a.c.KV;
@@ -307,9 +309,13 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
     s.s1 = min(s.s0 + (n << (plan.lg - 4)), (s.valid + 15) >> 4);
     un += n;
     rem -= n;
+    if (!waited && s.blk == (len - 1) >> 6) {
+      pdl_wait();
+      waited = true;
+    }
     const int64_t o = (int64_t)s.b * a.c.s_sb + (int64_t)s.kvh * a.c.s_sh + s.blk;
-    s.sk = a.c.ks[o];
-    s.sv = a.c.vs[o];
+    s.sk = __ldcg(a.c.ks + o);
+    s.sv = __ldcg(a.c.vs + o);
     return true;
   };
 
@@ -540,6 +546,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
   cp_wait<0>();
   last_pair = cur.b * KV + cur.kvh;
   }  // (warps with work)
+  if (!waited) pdl_wait();  // (what follows this kernel follows the append too)
 
   // ---- the last partials of the CTA's warps, joined where they are of one pair ----
   __syncthreads();  // the rings are empty
@@ -804,7 +811,7 @@ size_t kv8_decode_workspace_bytes(const b200mm_kv8& c, int B, int H) {
 }
 
 int kv8_decode(const b200mm_kv8& c, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-               int B, int H, Kv8Pos pos, float scale, void* ws, cudaStream_t st) {
+               int B, int H, Kv8Pos pos, float scale, void* ws, bool early, cudaStream_t st) {
   const bool fast = fast_shape(c, H) && !g_force_generic.load(std::memory_order_relaxed);
   const int esz = c.dtype == B200MM_F32 ? 4 : 2;
   for (int b0 = 0; b0 < B; b0 += kMaxRows) {
@@ -823,6 +830,7 @@ int kv8_decode(const b200mm_kv8& c, const void* q, int64_t q_sb, int64_t q_sh, v
     a.pos = pos;
     if (pos.dev) a.pos.dev += (int64_t)b0 * pos.stride;
     a.scale = scale;
+    a.early = early && b0 == 0;  // (a later launch follows the one before, with the same workspace)
     if (fast) {
       a.cw = cta_warps(c, H);
       a.W = split_ctas(c, a.B, a.cw) * a.cw;
