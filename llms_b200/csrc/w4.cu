@@ -230,6 +230,10 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
   float* red = reinterpret_cast<float*>(smem_raw + (size_t)nw * D * NM * MAT);
   const int rp = (M + 1) & ~1;
   const int red_n = NM * nw * 16 * rp;
+  // Columns 2 q, 2 q + 1 of a row.  Sums are read a column at a time: where 16 rows of rp would meet
+  // in two or four banks the pairs change places from row to row (16 rows of x: 33 -> 27 us).
+  const int zs = rp == 16 ? 1 : 2, zm = rp == 16 ? 7 : rp == 8 ? 3 : 0;
+  auto red_at = [&](int row, int q) { return row * rp + 2 * (q ^ ((row >> zs) & zm)); };
   const int xpitch = nsl * kSlice + 32;  // rows of x 64 bytes apart in the banks
   __half* xs = reinterpret_cast<__half*>(red + meet * red_n);             // [M][xpitch]
   float* xdown = reinterpret_cast<float*>(xs + (XREG ? 0 : (int64_t)M * xpitch));  // [nsl][8]: 1 / the slices' powers of two
@@ -466,7 +470,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
             for (int h = 0; h < 2; ++h)
               if (8 * t + 2 * c < M) {
                 const float d0 = XREG ? down[t][0] : 1.f, d1 = XREG ? down[t][1] : 1.f;
-                *reinterpret_cast<float2*>(mine + (mtx * nw * 16 + r + 8 * h) * rp + 8 * t + 2 * c) =
+                *reinterpret_cast<float2*>(mine + mtx * nw * 16 * rp + red_at(r + 8 * h, 4 * t + c)) =
                     make_float2(acc[mtx][t][2 * h] * d0, acc[mtx][t][2 * h + 1] * d1);
               }
         clear();
@@ -476,7 +480,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
           for (int o = threadIdx.x; o < (done - first) * 16 * M; o += blockDim.x) {
             const int row = o % 16, m = MT == 1 ? o / 16 % M : o / 16, tl = MT == 1 ? o / (16 * M) : 0;
             const int n = ((int)blockIdx.x + (first + tl) * (int)gridDim.x) * 16 + row;
-            const float* src = red + tl * red_n + row * rp + m;
+            const float* src = red + tl * red_n + red_at(row, m >> 1) + (m & 1);
             float v[NM];
 #pragma unroll
             for (int mtx = 0; mtx < NM; ++mtx) {
