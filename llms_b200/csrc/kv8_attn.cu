@@ -5,14 +5,14 @@
 // 16-bit cache costs, so the arithmetic per byte doubles; the kernel keeps the
 // stream in flight and the instructions per byte few:
 //   * a warp is on its own.  The flattened sequence of units (64 tokens, or 16
-//     where there are few) over (row, KV head, context) is cut into one
-//     contiguous range per warp, eight warps to a CTA and one CTA per SM.  The
+//     where there are too few of them) over (row, KV head, context) is cut into one
+//     contiguous range per warp, twelve warps to a CTA and one CTA per SM.  The
 //     lengths are read on the device, so one captured graph serves every
 //     position, and rows of any length share the machine evenly;
-//   * each warp fills a private ring of three slots with cp.async (K of a
-//     block, V of a block, alternately): two slots in flight while one is
-//     computed, 128 KB per SM, with no barrier between warps.  16-byte chunks
-//     are swizzled so that the fragment loads below meet no bank twice;
+//   * each warp has two slots of its own, for K and for V of a block, and fills
+//     each with cp.async for the next block as soon as it has used it: the other
+//     is in flight meanwhile, 96 to 192 KB per SM, with no barrier between warps.
+//     16-byte chunks are swizzled so that the fragment loads below meet no bank twice;
 //   * tokens are the rows of the matrix instructions (m16n8k16, fp16 x fp16 ->
 //     fp32) and the group's query heads the 8 columns: S[t, h] = K[t, d] Q[d, h]
 //     and O[d, h] = V^T[d, t] P[t, h].  8-bit values become fp16 exactly in
@@ -27,8 +27,17 @@
 //     that also carries the block's scale of V.
 // Each warp has one partial (max, sum, O) per (row, head) that its range touches.
 // Those of a CTA's warps that end in the same pair are joined in shared memory
-// (one long row of 8 KV heads: 18 partials per pair instead of 148, and 15 -> 4
-// us for the second kernel, which joins the rest).
+// (one long row of 8 KV heads: 18 partials per pair instead of 148 + 18), and a
+// second kernel joins the rest.
+//
+// Measured (B200, bf16, H 32, KV 8, D 128): 16 rows of 32768 tokens 166-174 us, 6.2
+// to 6.5 TB/s of cache; 32 rows of 4096 52 us (5.2 TB/s), of 1..4096 at random 32 us
+// (4.1); 1 row of 32768 22 us (3.0), of 512 8.6 us; the append adds 2 to 6 us to a step
+// (it runs beside the attention, but its CTAs and the attention's do not fit on
+// one SM).  Long contexts are bound by HBM (at 16 x 32768 the schedulers issue in 64 %
+// of the cycles, so not by much); short ones by what does not shrink: two dependent
+// launches, the plan, one block's latency and the joins, 8 us; those between
+// by whole blocks per warp (1 x 32768: 4096 blocks for 1776 warps, three rounds).
 //
 // Other shapes (fp32, head dims other than 64 / 128, more than 16 query heads
 // per KV head) run a kernel of one CTA per (head, row) on plain arithmetic.
@@ -38,8 +47,8 @@ namespace b200mm {
 
 namespace {
 
-constexpr int kThreads = 256;   // of the plain kernel
-constexpr int kWarps = kThreads / 32;
+constexpr int kGenericThreads = 256;
+constexpr int kGenericWarps = kGenericThreads / 32;
 constexpr int kMaxRows = 1024;  // rows of one launch (their lengths are summed by one CTA)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -52,7 +61,7 @@ struct AttnArgs {
   float scale;
   bool early;   // right behind the append of one token: only the rows' last blocks wait for it
   int W, cw;    // warps of the split kernel, and of a CTA of it
-  float* pacc;  // [W + B KV][g][D]: O, relative to the partial's max
+  float* pacc;  // [W + B KV][g][D]: sum of p v, relative to the partial's max
   float* pml;   // [W + B KV][g][2]: max (log2 units), sum
 };
 
@@ -62,8 +71,12 @@ struct AttnArgs {
 // warp i for pair p = row KV + head go to slot i + p, distinct for every (i, p)
 // that meet (ranges are contiguous); a warp that ends in the pair in which the
 // one before it in its CTA ends has its partial joined to that one's.  Units are
-// whole blocks where every warp has many, and 16 tokens below that, so that
-// short contexts spread over the SMs and the ranges are even.
+// whole blocks: a part of a block costs a warp nearly what the block does, so
+// finer ranges are even and no shorter (a step of 1 x 32768 with units of 16
+// tokens 27.3 us instead of 25.8, of 1 x 4096 15.5 instead of 12.2, of 32 x 2048
+// ragged 38.0 instead of 28.6).  Below a block for every fourth warp they are 16
+// tokens, so that short contexts spread over the SMs (1 x 512: 11.1 us, 12.2 with
+// blocks; 16 x 128: 14.5, 16.4).
 // (T fits 32 bits: 2^31 blocks would be 2 TB of cache.)
 struct Plan {
   int T, lg, W, per, more;  // per = T / W, more = T mod W
@@ -76,7 +89,7 @@ struct Plan {
 __device__ __forceinline__ int units(int len, int lg) { return (len + (1 << lg) - 1) >> lg; }
 __device__ __forceinline__ Plan make_plan(int64_t n64, int64_t n16, int W) {
   Plan p;
-  p.lg = n64 >= 8 * (int64_t)W ? 6 : 4;
+  p.lg = 4 * n64 >= (int64_t)W ? 6 : 4;
   p.T = (int)(p.lg == 6 ? n64 : n16);
   p.W = p.T < W ? p.T : W;
   p.per = p.W ? p.T / p.W : 0;
@@ -148,7 +161,8 @@ struct Seg {
 };
 
 // Warps per CTA: as many as the registers allow.  With eight the kernel waited
-// for its own instructions two thirds of the time (two warps per scheduler).
+// for its own instructions two thirds of the time (two warps per scheduler; 16
+// rows of 32768: 181 us a step, 172 with twelve).
 __host__ __device__ constexpr int split_warps(int NH) { return NH == 1 ? 12 : 8; }
 
 template <typename T, int D, int NH>
@@ -593,7 +607,8 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
 // ---------------------------------------------------------------------------
 // join: out[b, h] = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k over the
 // partials of the pair.  A warp per head, lane = 4 dims; a few partials each, so
-// no more threads, and nothing to wait for among them.
+// no more threads, and nothing to wait for among them (with a CTA per pair 32 x
+// 4096 ragged took 38 us instead of 36, both kernels).
 // ---------------------------------------------------------------------------
 constexpr int kJoinWarps = 4;
 
@@ -688,13 +703,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv8_join_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------------------
-// any shape: one CTA per (head, row), a warp per token, D <= 256
+// any shape: one CTA per (head, row), a warp per token, D <= 256.  For types and
+// dims that no served model of this package has; nothing is shared between the
+// heads of a group, so it reads the cache g times (from L2).
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(kThreads) kv8_generic_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kGenericThreads) kv8_generic_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int E = 8;  // dims per lane
-  __shared__ float acc_s[kWarps][256];
-  __shared__ float m_s[kWarps], l_s[kWarps];
+  __shared__ float acc_s[kGenericWarps][256];
+  __shared__ float m_s[kGenericWarps], l_s[kGenericWarps];
   const int h = blockIdx.x, b = blockIdx.y, kvh = h / a.g, D = a.c.D;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
@@ -711,7 +728,7 @@ __global__ void __launch_bounds__(kThreads) kv8_generic_kernel(const __grid_cons
     qv[e] = d < D ? to_f<T>(q[d]) : 0.f;
     acc[e] = 0.f;
   }
-  for (int64_t t = warp; t < len; t += kWarps) {
+  for (int64_t t = warp; t < len; t += kGenericWarps) {
     const int8_t* kr = a.c.kq + base + t * D;
     const int8_t* vr = a.c.vq + base + t * D;
     float s = 0.f;
@@ -737,9 +754,9 @@ __global__ void __launch_bounds__(kThreads) kv8_generic_kernel(const __grid_cons
   __syncthreads();
   if (threadIdx.x < D) {
     float mm = m_s[0];
-    for (int w = 1; w < kWarps; ++w) mm = fmaxf(mm, m_s[w]);
+    for (int w = 1; w < kGenericWarps; ++w) mm = fmaxf(mm, m_s[w]);
     float num = 0.f, den = 0.f;
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kGenericWarps; ++w) {
       const float f = m_s[w] == -INFINITY ? 0.f : exp2f(m_s[w] - mm);
       num += acc_s[w][threadIdx.x] * f;
       den += l_s[w] * f;
@@ -762,7 +779,7 @@ int split_ctas(const b200mm_kv8& c, int rows, int cw) {
 }
 
 template <typename T, int D, int NH>
-int launch_split(const AttnArgs& a) {
+int run_fast(const AttnArgs& a, cudaStream_t st) {
   constexpr size_t smem = (size_t)split_warps(NH) * 2 * 64 * D;
   auto kern = kv8_split_kernel<T, D, NH>;
   const int dev = current_device();
@@ -773,15 +790,7 @@ int launch_split(const AttnArgs& a) {
       return B200MM_ERR_LAUNCH;
     configured[dev] = true;
   }
-  return B200MM_OK;
-}
-
-template <typename T, int D, int NH>
-int run_fast(const AttnArgs& a, cudaStream_t st) {
-  const int s = launch_split<T, D, NH>(a);
-  if (s != B200MM_OK) return s;
-  constexpr size_t smem = (size_t)split_warps(NH) * 2 * 64 * D;
-  cudaError_t e = launch_pdl(kv8_split_kernel<T, D, NH>, dim3(a.W / a.cw), dim3(32 * a.cw), smem, st, a);
+  cudaError_t e = launch_pdl(kern, dim3(a.W / a.cw), dim3(32 * a.cw), smem, st, a);
   if (e != cudaSuccess) return B200MM_ERR_LAUNCH;
   e = launch_pdl(kv8_join_kernel<T>, dim3((a.H + kJoinWarps - 1) / kJoinWarps, a.B), dim3(32 * kJoinWarps), 0, st, a);
   return e == cudaSuccess ? B200MM_OK : B200MM_ERR_LAUNCH;
@@ -795,7 +804,7 @@ int run(const AttnArgs& a, bool fast, cudaStream_t st) {
       return a.g <= 8 ? run_fast<T, 64, 1>(a, st) : run_fast<T, 64, 2>(a, st);
     }
   }
-  return launch_pdl(kv8_generic_kernel<T>, dim3(a.H, a.B), dim3(kThreads), 0, st, a) == cudaSuccess
+  return launch_pdl(kv8_generic_kernel<T>, dim3(a.H, a.B), dim3(kGenericThreads), 0, st, a) == cudaSuccess
              ? B200MM_OK
              : B200MM_ERR_LAUNCH;
 }
