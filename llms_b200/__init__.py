@@ -3,7 +3,9 @@
 Subpackages / modules:
   kernels  -- fused QKV, fused gate-up-SiLU, int8 weight-only (reference
               ``src/kernels`` API), the ``o`` / ``down`` projections and the
-              GQA decode attention op for the engine's ``decode_attn_op`` seam
+              GQA decode attention op for the engine's ``decode_attn_op`` seam;
+              4-bit weights, the 8-bit KV cache and its attention, and log
+              probabilities of tokens
   mla      -- absorbed latent-KV MLA decode backend (reference
               ``engine/mla.py`` T == 1 branch), with the fused "Q + latent"
               projection of the decode step
