@@ -21,15 +21,18 @@
 // tokens) in registers between the maximum and the rounding, so each token is
 // read once.  Single tokens read the block's earlier tokens (at most 63 rows
 // from the tail) and write one row of 8 bits while the scale stands.
-// expand: 16 values per thread.  Both are streams, bound by HBM at length and
-// by one launch for single tokens.
+// expand: 16 values per thread.
+// Measured (B200, bf16, KV 8, D 128): 4096 tokens of one row in 9.3 us (25 MB moved,
+// 2.7 TB/s; 8 MB of it stay in L2) and out in 7.1 us, 4 x 1537 in 13.5 and 9.1.  The
+// append is bound by integer instructions (the maximum, the packing, the test for a
+// border: issue 66 %, special-function pipe 5 %), the expansion by the stream.
 #include "kv8.cuh"
 
 namespace b200mm {
 
 namespace {
 
-// 64 values per thread at D = 128: with 256 threads a third of the work was what each does once per block.
+// 64 values per thread at D = 128, 16-bit: with 256 threads a third of the work was what each does once per block.
 constexpr int kThreads = 128;
 
 struct AppendArgs {

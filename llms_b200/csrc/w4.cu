@@ -1,32 +1,38 @@
 // Projections with 4-bit weights and group scales:
 //   y[m, n] = epilogue(sum_k x[m, k] (u[n, k] - 8) s[n, k / G]),  G = 32, 64 or 128.
 //
-// Up to 64 rows of x the call is a stream of the weights (0.5 byte each), at
-// 13e12 weights a second on this GPU: one fp32 multiply-add per weight on the
-// CUDA cores would already take longer than the stream, so the products run on
-// mma.sync m16n8k16 from one row of x on, and what is left per weight is its
-// way from four bits to sixteen:
+// Up to 64 rows of x the weights (0.5 byte each) would stream at 13e12 a second
+// on this GPU: one fp32 multiply-add per weight on the CUDA cores would already
+// take longer, so the products run on mma.sync m16n8k16 from one row of x on, and
+// what is left per weight is its way from four bits to sixteen:
 //   * a warp owns 16 weight rows; lane l reads 16 bytes (32 weights) of rows
 //     l / 4 and l / 4 + 8 as they lie in memory, a chunk of 128 columns per warp;
 //   * the products of one instruction have to lie in one group, so for G = 64
 //     and 32 the four lanes of a row exchange words (one round of shuffles, or
 //     two: a 4 x 4 transpose).  The order of k inside a group is free: x is
 //     staged in shared memory in the order that the lanes hold the weights;
-//   * four bits under the exponent of 2^7 (bf16; 2^10 for fp16) are 128 + u:
-//     one logic instruction per pair, one packed subtraction, exact.  Pairs are
-//     the weights 4 apart in a 32-bit word;
+//   * four bits under the exponent of 2^10 (fp16; 2^7 for bf16 in the cluster kernel)
+//     are 1024 + u: one logic instruction per pair, one packed subtraction,
+//     exact.  Pairs are the weights 4 apart in a 32-bit word;
 //   * a group's products are summed in fp32 in accumulators of their own, which
 //     its scale then joins to the row's: no product is rounded;
 //   * before griddepcontrol.wait a CTA only asks for its first weights in L2.
 // Up to 16 rows of x, one persistent CTA per SM walks tiles of 16 weight rows.
 // Its warps split K; each has the part of x that it needs in registers (or, for
 // long K, x lies in shared memory) and fills a ring of its own with cp.async,
-// several tiles ahead, so only the sums of a tile meet at a barrier.  Otherwise K is split over a cluster of CTAs with 128 weight rows
-// each, and the sums meet in distributed shared memory.
+// several tiles ahead, so only the sums of a tile meet at a barrier.  Otherwise K
+// is split over a cluster of CTAs with 128 weight rows each, and the sums meet in
+// distributed shared memory (12288 x 4096 gate and up: one row 25 us there and 16 in the
+// persistent kernel, 16 rows 50 and 28).
 // From kDenseRows on the weights are expanded to 16 bits (rounded once: the
 // tcgen05 GEMM's operands are 16-bit) into the caller's workspace and the dense
-// GEMM takes them (12288 x 4096 gate and up: 113 us at 128 rows, where two
-// launches of 64 take 166; 83 us at 64 rows, where this would take 127).
+// GEMM takes them.  12288 x 4096 gate and up: 113 us at 128 rows, where two launches
+// of 64 take 165; 83 us at 64 rows, where this would take 127 (65 to 80 rows would
+// still be 100 to 112 in two launches, but 4096 x 12288 69 to 84 instead of 66).
+// Measured (cold weights, G = 128): 12288 x 4096 gate and up 15-16 us at one row (3.4
+// TB/s), 18 at 8, 28 at 16, 46 at 32; 6144 x 4096 6.1 us at one row, 10.9 at 16.  Not
+// HBM bounds these but instructions: issue slots half full, no pipe full, four warps
+// per scheduler.
 #include "w4.cuh"
 
 #include <type_traits>
@@ -511,7 +517,7 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const __grid_constant__ W4
   constexpr int WPG = 4 / GPC;         // words of a lane per group
   constexpr int RPO = kRows / CS;      // rows finished per CTA of the cluster
   constexpr int RP = MP + 2;           // pitch of the partial sums (even: float2 stores)
-  extern __shared__ __align__(16) unsigned char smem_raw[];
+  extern __shared__ __align__(128) unsigned char smem_raw[];
   const int xpitch = p.kslice + 32;    // elements: rows of x 64 bytes apart in the banks
   T* xs = reinterpret_cast<T*>(smem_raw);                                             // [MP][xpitch]
   float* red = reinterpret_cast<float*>(smem_raw + (size_t)MP * xpitch * sizeof(T));  // [NM][CS][RPO][RP]
@@ -747,8 +753,8 @@ int launch_stream(const W4Params& p, cudaStream_t st) {
     configured[dev] = true;
   }
   const int tiles = (p.N + 15) / 16, sms = num_sms(dev), grid = tiles < sms ? tiles : sms;
-  // the warps meet as rarely as shared memory allows (measured, one row: a meeting per tile costs the
-  // gate-up call 4 of its 17 us)
+  // the warps meet as rarely as shared memory allows (one row, gate-up: 16.8 us with a meeting per
+  // tile, 15.7 with one; 16 rows: fewer slots for three tiles a meeting took 29.8 instead of 28.1)
   int meet = MT == 1 ? (tiles + grid - 1) / grid : 1;
   while (meet > 1 && stream_smem(p.M, p.K, GATE, meet) > kStreamSmem) --meet;
   return launch_pdl(kern, dim3(grid), dim3(32 * stream_warps(p.K)), stream_smem(p.M, p.K, GATE, meet), st, p, meet) ==
