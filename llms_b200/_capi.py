@@ -268,7 +268,7 @@ def launch(name: str, t: torch.Tensor, *args) -> None:
     """Call entry point ``name`` with ``args`` and the current stream of ``t``'s
     device, on that device; raise on a non-zero status."""
     idx = t.device.index
-    if idx == torch.cuda.current_device():
+    if idx == torch._C._cuda_getDevice():
         st = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
@@ -283,7 +283,7 @@ def launch_count() -> int:
 
 def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError(
                 "b200mm kernels run on CUDA (sm_100a) tensors only; got a tensor on "
                 f"{t.device}. There is no CPU path."

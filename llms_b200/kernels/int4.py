@@ -110,7 +110,7 @@ def int4_fused_qkv(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, *, n_q: in
     """``x @ W_qkv.T`` split into q / k / v views of one buffer; as ``int8_fused_qkv``."""
     if n_q + 2 * n_k != w.shape[0]:
         raise ValueError(f"n_q + 2*n_k ({n_q} + 2*{n_k} = {n_q + 2 * n_k}) != W_qkv.shape[0] ({w.shape[0]})")
-    return int4_linear(x, w, s).split([n_q, n_k, n_k], dim=-1)
+    return torch.split_with_sizes(int4_linear(x, w, s), (n_q, n_k, n_k), -1)
 
 
 def int4_fused_gate_up_silu(x: torch.Tensor, wg: torch.Tensor, sg: torch.Tensor, wu: torch.Tensor,

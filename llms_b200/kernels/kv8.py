@@ -222,7 +222,7 @@ def int8_kv_decode_attn(q: torch.Tensor, kv: Int8KV, pos: int | torch.Tensor, *,
     _check_host_pos(kv, pos, 1)
     B, H, _, D = q.shape
     host, dev, stride = _pos(pos, B, kv.device)
-    out = q.new_empty((B, H, 1, D))
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, 1, D))
     if B == 0:
         return out
     q = _aligned(q)
@@ -244,7 +244,7 @@ def int8_kv_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: Int8KV, 
         raise ValueError(f"k {tuple(k.shape)} must hold one token for each of q's {B} rows")
     _check_host_pos(kv, pos, 1)
     host, dev, stride = _pos(pos, B, kv.device)
-    out = q.new_empty((B, H, 1, D))
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, 1, D))
     if B == 0:
         return out
     q, k, v = _aligned(q), _aligned(k), _aligned(v)

@@ -52,10 +52,11 @@ def b200_token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int 
         x = x.contiguous()
     M = x.shape[0]
     lead = logits.shape[:-1]
-    lp, ent = x.new_empty(lead, dtype=torch.float32), x.new_empty(lead, dtype=torch.float32)
-    ids, lps = x.new_empty((*lead, top), dtype=torch.int64), x.new_empty((*lead, top), dtype=torch.float32)
+    toks = tokens if tokens.is_contiguous() else tokens.contiguous()
+    lp = x.new_empty(lead, dtype=torch.float32)
+    ent, ids = torch.empty_like(lp), toks.new_empty((*lead, top))
+    lps = lp.new_empty((*lead, top))
     if M:
-        toks = tokens.contiguous()
         _capi.launch("b200mm_token_logprobs", x, x.data_ptr(), x.stride(0) if M > 1 else V, toks.data_ptr(), lp.data_ptr(), ent.data_ptr(),
                      ids.data_ptr(), lps.data_ptr(), M, V, top, code)
     return TokenLogprobs(lp, ent, ids, lps)
