@@ -179,7 +179,8 @@ def int8_kv_expand(kv: Int8KV, length: int, *, batch: int | None = None) -> tupl
         raise ValueError(f"length {length}, batch {B} do not fit a cache of {tuple(kv.kq.shape)}")
     _capi.require_cuda(kv.kq)
     shape = (B, kv.num_kv_heads, length, kv.head_dim)
-    k, v = kv.kt.new_empty(shape), kv.kt.new_empty(shape)
+    k = kv.kt.new_empty(shape)
+    v = torch.empty_like(k)
     if k.numel():
         _capi.launch("b200mm_kv8_expand", k, kv._ref, k.data_ptr(), v.data_ptr(), *k.stride()[:3], B, length)
     return k, v
