@@ -18,7 +18,7 @@ struct Kv8Pos {
   const int64_t* dev;
   int64_t host;
   int stride;
-  __device__ __forceinline__ int64_t operator()(int b) const { return dev ? dev[(int64_t)b * stride] : host; }
+  __device__ __forceinline__ int64_t operator()(int b) const { return dev ? __ldcg(dev + (int64_t)b * stride) : host; }
 };
 
 // Tokens that row b attends to, for its last position p: p + 1, at most the capacity; none below 0.

@@ -176,6 +176,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
   extern __shared__ __align__(1024) unsigned char ring[];
   constexpr int PT = (kMaxRows + kThreads - 1) / kThreads;
   __shared__ int pre[PT * kThreads + 1];  // units of one head in rows before b
+  __shared__ int lens[PT * kThreads];     // tokens of row b
   __shared__ long long red[2][kWarps];
   __shared__ int last_s[kWarps];        // the pair that a warp's range ends in
 
@@ -184,18 +185,18 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
   const uint32_t none = (uint32_t)a.B >> 31;  // 0, unknown to the compiler
   const uint32_t mask = 0x00ff00ffu + none, bits = 0x64806480u + none;
   pdl_trigger();
-  bool waited = !a.early;
+  bool waited = !a.early;  // (until then everything is read past L1, which the kernel before may still fill)
   if (waited) pdl_wait();
 
   // the plan: lengths summed over the rows; one position for all rows needs no sum
   const int KV = a.c.KV;
   const bool even = a.pos.stride == 0;
   Plan plan;
-  int nu0 = 0;  // units of a head, one position for all
+  int nu0 = 0, len0 = 0;  // units of a head and tokens, one position for all
   if (even) {
-    const int len = kv8_len(a.pos(0), a.c.S);
-    plan = make_plan((int64_t)a.B * KV * units(len, 6), (int64_t)a.B * KV * units(len, 4), a.W);
-    nu0 = units(len, plan.lg);
+    len0 = kv8_len(a.pos(0), a.c.S);
+    plan = make_plan((int64_t)a.B * KV * units(len0, 6), (int64_t)a.B * KV * units(len0, 4), a.W);
+    nu0 = units(len0, plan.lg);
   } else {
     int len[PT];
     long long n64 = 0, n16 = 0;
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       pre[threadIdx.x * PT + i] = base;
+      lens[threadIdx.x * PT + i] = len[i];
       base += units(len[i], plan.lg);
     }
     if (threadIdx.x == kThreads - 1) pre[PT * kThreads] = base;
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
     nh = v / nu;
     un = v - nh * nu;
   }
-  len = kv8_len(a.pos(nb), a.c.S);
+  len = even ? len0 : lens[nb];
   auto next_seg = [&](Seg& s) -> bool {
     if (rem <= 0) return false;
     if (un == nu) {  // next pair; rows without tokens have none
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
         if (!even) {
           while (pre[nb + 1] == pre[nb]) ++nb;
           nu = pre[nb + 1] - pre[nb];
-          len = kv8_len(a.pos(nb), a.c.S);
+          len = lens[nb];
         }
       }
     }
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (h < a.g) v = *reinterpret_cast<const uint4*>(qp + 64 * j + 8 * e);
+          if (h < a.g) v = __ldcg(reinterpret_cast<const uint4*>(qp + 64 * j + 8 * e));
           Chunk<T>::unpack(v, &f[j][8 * e]);
         }
 #pragma unroll

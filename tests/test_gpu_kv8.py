@@ -449,3 +449,44 @@ def test_empty_calls():
     assert int8_kv_decode_attn(torch.zeros(0, 4, 1, 64, dtype=BF, device="cuda"), kv, 0, scale=0.1).shape == (0, 4, 1, 64)
     k, v = int8_kv_expand(kv, 0)
     assert k.shape == (2, 2, 0, 64) == v.shape
+
+
+@pytest.mark.parametrize("B,L", [(1, 64), (1, 5000), (5, 640), (40, 1217)])
+def test_a_step_right_behind_what_it_reads(B, L):
+    """The step's attention starts before its append is done, but not before the
+    prompt's append (or the copies of q, k, v) right ahead of it: eager, and
+    in a graph whose inputs change between replays."""
+    from llms_b200.kernels import int8_kv_append, int8_kv_decode_attn, int8_kv_step
+    S = L + 1
+    a, b = _alloc(B, 8, S, 128), _alloc(B, 8, S, 128)
+    pos = torch.full((B,), L, dtype=torch.int64, device="cuda")
+    pos[B // 2] = L - 1 if B > 1 else L  # (written anew)
+    data = []
+    for i in range(6):
+        k, v = _tokens(B, 8, S, 128, seed=40 + i)
+        q = torch.randn(B, 32, 1, 128, device="cuda").to(BF)
+        int8_kv_append(b, k[:, :, :L], v[:, :, :L], 0)
+        torch.cuda.synchronize()
+        int8_kv_append(b, k[:, :, L:], v[:, :, L:], pos)
+        torch.cuda.synchronize()
+        data.append((q, k, v, int8_kv_decode_attn(q, b, pos, scale=0.09)))
+    q, k, v = (torch.zeros_like(x) for x in data[0][:3])
+
+    def run():
+        int8_kv_append(a, k[:, :, :L], v[:, :, :L], 0)
+        return int8_kv_step(q, k[:, :, L:], v[:, :, L:], a, pos, scale=0.09)
+
+    run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    for graph in (False, True):
+        for dq, dk, dv, want in data * 3:
+            q.copy_(dq), k.copy_(dk), v.copy_(dv)
+            if graph:
+                g.replay()
+                got = out
+            else:
+                got = run()
+            assert torch.equal(got, want)
