@@ -21,10 +21,15 @@
 //     from two rows by the byte permute that widens them;
 //   * q is scaled per head by a power of two that brings its largest element
 //     into [2^14, 2^15): bf16 -> fp16 is then exact to 2^-38 of that element;
-//   * the softmax is local to a block: p = 2^(s - max of the block + 14),
-//     rounded to fp16 (11 bits, and 2^-38 of the block's largest still counts),
-//     the block's O in fp32, joined to the running sums with one factor
-//     that also carries the block's scale of V.
+//   * the softmax is local to a block: p = 2^(s - max of the block + 14), held
+//     as two fp16 numbers, p rounded and what that left (22 bits; 2^-39 of the
+//     block's largest still counts), each with its own matrix instruction into
+//     the block's O in fp32, which is joined to the running sums with one factor
+//     that also carries the block's scale of V.  (p in one fp16 number would cost the
+//     outputs as much as their own rounding to fp16 does: with it a norm of 2.5e-4
+//     off the formula instead of 2.1e-4, of which 2.1e-4 are the outputs' rounding.
+//     The second number costs 2 to 4 % of a step that the stream does not bound, 1 x
+//     16384 20.1 -> 20.7 us, and nothing at 16 x 32768.)
 // Each warp has one partial (max, sum, O) per (row, head) that its range touches.
 // Those of a CTA's warps that end in the same pair are joined in shared memory
 // (one long row of 8 KV heads: 18 partials per pair instead of 148 + 18), and a
@@ -453,7 +458,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
           for (int e = 0; e < 4; ++e)
             if (s < cur.s0 || s >= cur.s1 || 16 * s + r + 8 * (e >> 1) >= cur.valid) sc[n][s][e] = -INFINITY;
     }
-    uint32_t pf[NH][4][2];
+    uint32_t pf[NH][4][2], pr[NH][4][2];  // p in fp16, and what the rounding left, in fp16 too
     float fo[NH][2], fb[NH][2];  // factors of the running and of the block's sums
     bool same = true;            // no maximum moved
 #pragma unroll
@@ -488,8 +493,13 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
           if (!all && sc[n][s][e] == -INFINITY) p[e] = 0.f;  // (a factor of 0 would make it NaN: a block of zero keys)
           lb[e & 1] += p[e];
         }
-        pf[n][s][0] = transpose8x8(pack_h2(p[0], p[1]));  // tokens 2c, 2c + 1 of head r
-        pf[n][s][1] = transpose8x8(pack_h2(p[2], p[3]));  // tokens 2c + 8, 2c + 9
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // tokens 2c, 2c + 1 of head r, tokens 2c + 8, 2c + 9
+          const uint32_t h = pack_h2(p[2 * e], p[2 * e + 1]);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          pf[n][s][e] = transpose8x8(h);
+          pr[n][s][e] = transpose8x8(pack_h2(p[2 * e] - f.x, p[2 * e + 1] - f.y));
+        }
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -534,7 +544,10 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
             const uint32_t a0 = i8_pair_to_h2(v0[w], v1[w], k, mask, bits), a1 = i8_pair_to_h2(v0[w], v1[w], k + 1, mask, bits);
             const uint32_t a2 = i8_pair_to_h2(v8[w], v9[w], k, mask, bits), a3 = i8_pair_to_h2(v8[w], v9[w], k + 1, mask, bits);
 #pragma unroll
-            for (int n = 0; n < NH; ++n) mma_h(ob[n][i], a0, a1, a2, a3, pf[n][s][0], pf[n][s][1]);
+            for (int n = 0; n < NH; ++n) {
+              mma_h(ob[n][i], a0, a1, a2, a3, pf[n][s][0], pf[n][s][1]);
+              mma_h(ob[n][i], a0, a1, a2, a3, pr[n][s][0], pr[n][s][1]);
+            }
           }
         }
       }

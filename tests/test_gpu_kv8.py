@@ -490,3 +490,51 @@ def test_a_step_right_behind_what_it_reads(B, L):
             else:
                 got = run()
             assert torch.equal(got, want)
+
+
+def _against(p, part):
+    """Signs (T,) that add up what rounding each of p (times 2^14, relative to the largest of its part) to fp16
+    leaves, and sum to zero with p as weights: the tokens that leave least are spent on that."""
+    u = torch.nn.functional.pad(p, (0, -len(p) % part)).view(-1, part)
+    m = u.amax(-1, keepdim=True)
+    left = ((u / m * 2.0 ** 14).half().double() * 2.0 ** -14 * m - u).flatten()[:len(p)]
+    sign = torch.where(left > 0, 1.0, -1.0).double()
+    free = left.abs().argsort()[:len(p) // 2]
+    sign[free] = 0
+    total = (sign * p).sum().item()
+    for i in free[p[free].argsort(descending=True)].tolist():
+        sign[i] = 1.0 if total < 0 else -1.0
+        total += sign[i].item() * p[i].item()
+    return sign
+
+
+@pytest.mark.parametrize("B,H,KV,D,L,S,part", [(1, 1, 1, 128, 400, 4096, 16), (4, 32, 8, 128, 1000, 1000, 64), (2, 16, 1, 64, 900, 900, 64),
+                                               (3, 24, 2, 128, 300, 4096, 16), (4, 40, 8, 64, 1000, 1000, 64)])
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_probabilities_are_not_cut_to_16_bits(dtype, B, H, KV, D, L, S, part):
+    """Values that follow the sign of what rounding a probability to fp16 would
+    leave, for one head of each group.  The bound, relative to the mass
+    sum_t p_t |v_t|, twice (the products' sum and the one it is divided by): a
+    score is the sum of D / 16 instructions' results, each within 2^-23 of A =
+    max_t sum_d |q_d k_d| scale, times factors rounded four times; the
+    exponential and the held probability are within 2^-22 each; 8 products of a
+    part and the 3 roundings of each join.  Then 2^-39 of every |v| (see the head
+    of this file) and half a step of the output."""
+    from llms_b200.kernels import int8_kv_append, int8_kv_decode_attn
+    kv = _alloc(B, KV, S, D, dtype)
+    k = _tokens(B, KV, L, D, dtype, seed=H + L)[0]
+    int8_kv_append(kv, k, k, 0)
+    q = torch.randn(B, H, 1, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).to(dtype)
+    scale = D ** -0.5
+    held = (kv.kq.double() * kv.ks.double().repeat_interleave(64, 2)[..., None])[:, :, :L]
+    p = torch.exp((q.double()[:, ::H // KV] @ held.transpose(-1, -2))[:, :, 0] * scale).cpu()
+    v = torch.stack([torch.stack([_against(p[b, h], part) for h in range(KV)]) for b in range(B)])
+    int8_kv_append(kv, k, v.to("cuda", dtype)[..., None].expand(B, KV, L, D), 0)
+    got = int8_kv_decode_attn(q, kv, L - 1, scale=scale)
+    want, mass, every = _attend(q, kv, [L] * B, scale)
+    A = (q.double().abs() @ held.abs().repeat_interleave(H // KV, 1).transpose(-1, -2)).amax().item() * scale
+    rel = 2 * ((D / 16 + 4) * A * 2.0 ** -23 + 2 * 2.0 ** -22 + (8 + 3 * L / part) * 2.0 ** -23)
+    assert rel < 2.0 ** -13.8  # (cut probabilities: about 2^-13)
+    tol = rel * mass + 2.0 ** -39 * every + torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -25 if dtype == HF else 0)
+    d = (got[:, :, 0].double() - want).abs() - tol
+    assert (d <= 0).all(), f"off by {d.max().item():.3e} beyond {tol.flatten()[d.argmax()].item():.3e}"
