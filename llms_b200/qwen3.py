@@ -346,11 +346,17 @@ class GraphedDecodeStep:
     ``logits = step(ids, pos)`` for each new token (ids: (batch, 1) on the
     device).  The returned logits live in a static buffer overwritten by the
     next call.  Building the graph runs the step once at ``cache.cur_len``,
-    the row the first real step writes anyway."""
+    the row the first real step writes anyway.  Positions lie inside the cache
+    and inside the model's RoPE tables (an 8-bit cache's capacity, whole blocks of
+    64, may reach further): on the device nothing would stop one beyond them."""
 
     def __init__(self, model: Qwen3Model, kv_cache: KVCache, batch: int) -> None:
         dev = model.embed.weight.device
         self.model, self.cache = model, kv_cache
+        # (an 8-bit cache that is full drops the token of the run below)
+        room = model.rope_cos.shape[0] if isinstance(kv_cache, Int8KVCache) else self._positions()
+        if not 0 <= kv_cache.cur_len < room:
+            raise ValueError(f"no room for a step at position {kv_cache.cur_len} (rows 0..{room - 1})")
         self.ids = torch.zeros(batch, 1, dtype=torch.long, device=dev)
         self.pos = torch.full((1,), kv_cache.cur_len, dtype=torch.long, device=dev)
         s = torch.cuda.Stream(dev)
@@ -365,11 +371,16 @@ class GraphedDecodeStep:
         with torch.cuda.graph(self.graph), torch.inference_mode():
             self.logits = model.forward_static(self.ids, kv_cache, self.pos)
 
+    def _positions(self) -> int:
+        """How many positions both the cache and the RoPE tables have."""
+        S = self.cache.capacity if isinstance(self.cache, Int8KVCache) else self.cache.k[0].shape[2]
+        return min(S, self.model.rope_cos.shape[0])
+
     def __call__(self, ids: torch.Tensor, pos: int) -> torch.Tensor:
         int8 = isinstance(self.cache, Int8KVCache)
-        S = self.cache.capacity if int8 else self.cache.k[0].shape[2]
+        S = self._positions()
         if not 0 <= pos < S:
-            raise ValueError(f"position {pos} is outside the cache (rows 0..{S - 1})")
+            raise ValueError(f"position {pos} is outside the cache and the model's positions (rows 0..{S - 1})")
         if tuple(ids.shape) != tuple(self.ids.shape):
             raise ValueError(f"ids shape {tuple(ids.shape)} != the captured step's {tuple(self.ids.shape)}")
         if int8:

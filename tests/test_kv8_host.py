@@ -175,3 +175,46 @@ def test_going_back_twice_refills_the_open_block():
         kv.kt[0, 0, :40] = 9
         c.seek(10)  # inside the block that is open now
         assert (kv.kt[0, 0, :40] == 9).all() and c.cur_len == 10 == kv.length
+
+
+def _captured_step(max_positions, cache_of):
+    """A GraphedDecodeStep without its graph (no GPU here): replays are counted."""
+    import types
+
+    from llms_b200.qwen3 import GraphedDecodeStep, Qwen3Model, Qwen3Shape
+    model = Qwen3Model(Qwen3Shape(vocab_size=8, hidden_size=32, num_hidden_layers=2, num_attention_heads=2, num_key_value_heads=2,
+                                  head_dim=16, intermediate_size=32, max_position_embeddings=max_positions))
+    step = GraphedDecodeStep.__new__(GraphedDecodeStep)
+    step.model, step.cache, step.replays = model, cache_of(model), 0
+
+    def replay():
+        step.replays += 1
+
+    step.graph, step.logits = types.SimpleNamespace(replay=replay), torch.zeros(1, 1, 8)
+    step.ids, step.pos = torch.zeros(1, 1, dtype=torch.long), torch.zeros(1, dtype=torch.long)
+    return step
+
+
+@pytest.mark.parametrize("int8,size", [(True, 100), (False, 128)])
+def test_a_captured_step_stays_inside_the_rope_tables(int8, size):
+    """100 positions, and a cache that reaches further (8-bit: two blocks of 64)."""
+    from llms_b200.qwen3 import GraphedDecodeStep
+    step = _captured_step(100, lambda m: m.alloc_cache(size, int8=int8))
+    ids = torch.ones(1, 1, dtype=torch.long)
+    step.cache.cur_len = 99
+    step(ids, 99)
+    assert step.replays == 1 and step.cache.cur_len == 100 and step.pos.item() == 99
+    for pos in (100, 127, 128, -1):
+        with pytest.raises(ValueError):
+            step(ids, pos)
+    assert step.replays == 1
+    with pytest.raises(ValueError, match="no room"):  # building it would run a step at 100
+        GraphedDecodeStep(step.model, step.cache, 1)
+
+
+def test_a_step_is_not_captured_on_a_full_16_bit_cache():
+    from llms_b200.qwen3 import GraphedDecodeStep
+    step = _captured_step(100, lambda m: m.alloc_cache(40))
+    step.cache.cur_len = 40
+    with pytest.raises(ValueError, match="no room"):
+        GraphedDecodeStep(step.model, step.cache, 1)
