@@ -98,12 +98,16 @@ class Int8KV:
     def length(self, n: int) -> None:  # by an append that ended at n
         self._length, self._tail = n, (n - 1) // KV8_BLOCK  # (the block that kt, vt hold)
 
+    def _check_rewind(self, n: int) -> None:
+        if not 0 <= n <= self._length:
+            raise ValueError(f"cannot go to position {n}: the cache holds {self._length} tokens")
+
+    @torch.inference_mode()  # (a cache made in inference mode may be written in no other)
     def rewind(self, n: int) -> None:
         """Forget the tokens from position ``n`` on.  Inside the block that the
         last append ended in the tokens are still there as they came; further
         back the open block's tokens are taken from their 8-bit values."""
-        if not 0 <= n <= self._length:
-            raise ValueError(f"cannot go to position {n}: the cache holds {self._length} tokens")
+        self._check_rewind(n)
         blk, r = divmod(n, KV8_BLOCK)
         if r and blk != self._tail:
             for q, s, t in ((self.kq, self.ks, self.kt), (self.vq, self.vs, self.vt)):
@@ -284,6 +288,8 @@ class Int8KVCache:
     def cur_len(self, n: int) -> None:
         """Up: tokens that a captured step has put in.  Down: :meth:`seek`."""
         for layer in self.layers:
+            layer._check_rewind(min(n, layer.length))
+        for layer in self.layers:
             if n > layer.length:
                 layer.length = n
             elif n < layer.length:
@@ -293,6 +299,8 @@ class Int8KVCache:
     def seek(self, pos: int) -> None:
         """Make ``pos`` the next position of every layer: where the tokens end,
         or before (the tokens from there on are forgotten)."""
+        for layer in self.layers:  # all or none
+            layer._check_rewind(pos)
         for layer in self.layers:
             if pos != layer.length:
                 layer.rewind(pos)

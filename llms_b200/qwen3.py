@@ -376,6 +376,7 @@ class GraphedDecodeStep:
         S = self.cache.capacity if isinstance(self.cache, Int8KVCache) else self.cache.k[0].shape[2]
         return min(S, self.model.rope_cos.shape[0])
 
+    @torch.inference_mode()
     def __call__(self, ids: torch.Tensor, pos: int) -> torch.Tensor:
         int8 = isinstance(self.cache, Int8KVCache)
         S = self._positions()

@@ -218,3 +218,41 @@ def test_a_step_is_not_captured_on_a_full_16_bit_cache():
     step.cache.cur_len = 40
     with pytest.raises(ValueError, match="no room"):
         GraphedDecodeStep(step.model, step.cache, 1)
+
+
+def _inference_cache(model):
+    with torch.inference_mode():
+        return model.alloc_cache(192, int8=True)
+
+
+def test_a_cache_of_inference_tensors_goes_back_outside_inference_mode():
+    step = _captured_step(192, _inference_cache)
+    c = step.cache
+    c.cur_len = 150
+    with torch.inference_mode():
+        for layer in c.layers:
+            layer.kq.fill_(3), layer.ks.fill_(0.5), layer.kt.fill_(7)
+    step(torch.ones(1, 1, dtype=torch.long), 100)  # the block before the open one
+    assert c.cur_len == 101 and step.replays == 1
+    assert all((x.kt[:, :, :36] == 1.5).all() and (x.kt[:, :, 36:] == 7).all() for x in c.layers)
+    c.cur_len = 20
+    c.seek(10)
+    c.layers[0].rewind(5)
+    assert all((x.kt[:, :, :20] == 1.5).all() for x in c.layers)
+
+
+def test_a_step_built_in_inference_mode_is_called_outside():
+    with torch.inference_mode():
+        step = _captured_step(64, lambda m: m.alloc_cache(64))
+    step(torch.ones(1, 1, dtype=torch.long), 3)
+    assert step.replays == 1 and step.ids.item() == 1 and step.pos.item() == 3
+
+
+def test_a_refused_seek_leaves_every_layer_where_it_was():
+    c = Int8KVCache.alloc(num_layers=3, max_batch=1, num_kv_heads=1, max_seq_len=128, head_dim=64, dtype=torch.float16, device="cpu")
+    c.cur_len = 100
+    c.layers[2].rewind(70)  # (a forward that failed between layers)
+    for move in (lambda: c.seek(90), lambda: c.seek(-1), lambda: setattr(c, "cur_len", -1)):
+        with pytest.raises(ValueError):
+            move()
+        assert [x.length for x in c.layers] == [100, 100, 70] and c.cur_len == 100
