@@ -149,15 +149,21 @@ __device__ __forceinline__ void cp_wait() {
 // Ring slots per warp (2 KB of each matrix a slot).
 __host__ __device__ constexpr int stream_depth(bool gate, bool xreg) { return (xreg ? 6 : 4) / (gate ? 2 : 1); }
 
-// The eight weights of a word as four fp16 pairs, (0, 4), (1, 5), (2, 6), (3, 7):
+// The eight weights of a word as four pairs, (0, 4), (1, 5), (2, 6), (3, 7).  fp16:
 // under the exponent of 2^10 a low half is 1024 + u, a high half 1024 + 16 u, so
-// one shift serves two logic instructions (bf16's 7 bits would want one each).
+// one shift serves two logic instructions (bf16's 7 bits want one each).
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
   uint32_t v;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(mask), "r"(bits));
   return v;
 }
-__device__ __forceinline__ void nibbles_h2(uint32_t w, uint32_t (&o)[4]) {
+template <typename W>
+__device__ __forceinline__ void nibbles(uint32_t w, uint32_t (&o)[4]) {
+  if constexpr (std::is_same<W, __nv_bfloat16>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = Nib<W>::pair(w, i);
+    return;
+  }
   const __half2 low = __float2half2_rn(-1032.f), k = __float2half2_rn(0.0625f), high = __float2half2_rn(-72.f);
   uint32_t v[4] = {and_or(w, 0x000f000fu, 0x64006400u), and_or(w, 0x00f000f0u, 0x64006400u),
                    and_or(w >> 8, 0x000f000fu, 0x64006400u), and_or(w >> 8, 0x00f000f0u, 0x64006400u)};
@@ -169,12 +175,10 @@ __device__ __forceinline__ void nibbles_h2(uint32_t w, uint32_t (&o)[4]) {
   }
 }
 
-// Eight values of x as fp16, times `up` (bf16; fp16 as they are), in the order of a word's pairs.
-template <typename T>
-__device__ __forceinline__ uint4 x_pairs(const uint4& v, float up) {
-  if constexpr (std::is_same<T, __half>::value) return pair_order(v);
+// Eight bf16 values of x as fp16, times `up`, in the order of a word's pairs.
+__device__ __forceinline__ uint4 scaled_pairs(const uint4& v, float up) {
   float f[8];
-  Chunk<T>::unpack(v, f);
+  Chunk<__nv_bfloat16>::unpack(v, f);
   uint32_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -183,14 +187,29 @@ __device__ __forceinline__ uint4 x_pairs(const uint4& v, float up) {
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
-template <typename T>
-__device__ __forceinline__ float x_max(const uint4& v) {
-  float f[8], m = 0.f;
-  Chunk<T>::unpack(v, f);
+// Magnitudes of bf16 values, as their bits, two at a time: the largest and the smallest ...
+struct Spread {
+  uint32_t most = 0, least = ~0u;
+  __device__ __forceinline__ void take(const uint4& v) {
+    const uint32_t m = 0x7fff7fffu, a = v.x & m, b = v.y & m, c = v.z & m, d = v.w & m;
+    most = __vmaxu2(most, __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d)));
+    least = __vminu2(least, __vminu2(__vminu2(a, b), __vminu2(c, d)));
+  }
+  __device__ __forceinline__ uint32_t largest() const { return max(most >> 16, most & 0xffffu); }
+  __device__ __forceinline__ uint32_t smallest() const { return min(least >> 16, least & 0xffffu); }
+};
+// ... and bits 15 and 31 set in `lost` where one is not zero and below `least`.  (a + 0x7fff has
+// bit 15 set from a = 1 on, a + 0x8000 - least from a = least on; no half carries into the next.)
+__device__ __forceinline__ uint32_t below(const uint4& v, uint32_t least, uint32_t lost) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w}, m = 0x7fff7fffu, k = 0x80008000u - least * 0x00010001u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
-  return m;
+  for (int i = 0; i < 4; ++i) lost |= ((w[i] & m) + m) & ~((w[i] & m) + k);
+  return lost;
 }
+// fp16 with the largest below 2^15 holds 8 bits from 2^-17 on: exponents at most 31 apart
+// (below the normal numbers, where steps no longer shrink, the last normal one's counts).
+__device__ __forceinline__ uint32_t least_bits(uint32_t most) { return most < 33u << 7 ? 0u : ((most >> 7) - 31) << 7; }
+__device__ __forceinline__ float bf16_value(uint32_t bits) { return __uint_as_float(bits << 16); }
 // The power of two that brings `mx` into [2^14, 2^15), and its inverse (both normal).
 __device__ __forceinline__ float x_up(float mx, float& down) {
   const int e = max(1, min(268 - (int)(__float_as_uint(mx) >> 23), 253));
@@ -204,15 +223,20 @@ __device__ __forceinline__ float scale_of(uint32_t bits) {
   return to_f<T>(*reinterpret_cast<const T*>(&h));
 }
 
-// Products are fp16 x fp16: bf16 rows of x are scaled by a power of two per
-// slice of K that brings the largest element into [2^14, 2^15), so they are
-// exact down to 2^-29 of it and within 2^-39 of it below; the sums are scaled back.
+// Products are exact.  fp16 weights take fewer instructions to widen than bf16 ones
+// (12288 x 4096 gate and up, one row: 16.1 us, 18.9 with bf16), so up to 8 bf16 rows
+// of x become fp16 too, by a power of two per slice of K and row that brings the
+// largest element into [2^14, 2^15) and that the sums are scaled back by.  Where one
+// of a slice's elements would lose bits that way (its exponent lies more than 31
+// below the largest) the products are in bf16; looking for one costs 0.4 us.  (9 to
+// 16 rows 27.3 and 28.0 us, 6144 x 4096 10.2 and 9.6: bf16 there, without the factors'
+// registers.)
 // XREG: every warp has one slice of K, and its part of x stays in registers;
 // otherwise all of x is staged in shared memory.
 template <typename T, int MT, int G, bool GATE, bool XREG>
 __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const __grid_constant__ W4Params p, const int meet_tiles) {
   const int meet = MT == 1 ? meet_tiles : 1;  // (16 rows: no room for more than one, nor registers to count them)
-  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool HALF = std::is_same<T, __nv_bfloat16>::value && MT == 1;  // bf16 x as fp16 where that is exact
   constexpr int NM = GATE ? 2 : 1;
   constexpr int D = stream_depth(GATE, XREG);
   constexpr int GPC = kChunk / G;  // groups per chunk
@@ -330,11 +354,12 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
   const T* x = static_cast<const T*>(p.x);
   uint4 xr[XREG ? 2 : 1][4][MT];  // of the warp's slice: chunk, word, n-tile
   float down[MT][2];              // of columns 8 t + 2 c, + 1
+  bool wide = false;              // bf16 products (XREG: in this warp, otherwise in the CTA)
   if constexpr (XREG) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       const int m = r + 8 * t;
-      float mx = 0.f;
+      Spread sp;
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
@@ -342,38 +367,60 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
           const int k = warp * kSlice + hh * kChunk + word_col<G>(j, c);
           xr[hh][j][t] = make_uint4(0, 0, 0, 0);
           if (m < M && k < K) xr[hh][j][t] = *reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k);
-          if constexpr (BF) mx = fmaxf(mx, x_max<T>(xr[hh][j][t]));
+          if constexpr (HALF) sp.take(xr[hh][j][t]);
         }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      float dn;
-      const float up = x_up(mx, dn);
+      float up = 1.f, dn = 1.f;
+      if constexpr (HALF) {
+        uint32_t most = sp.largest();
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        if (__any_sync(0xffffffffu, m < M && sp.smallest() < least_bits(most))) {  // a zero, or less
+          uint32_t lost = 0;
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) lost = below(xr[hh][j][t], least_bits(most), lost);
+          wide = __any_sync(0xffffffffu, lost & 0x80008000u);
+        }
+        if (!wide) up = x_up(bf16_value(most), dn);
+      }
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) xr[hh][j][t] = x_pairs<T>(xr[hh][j][t], up);
-      down[t][0] = BF ? __shfl_sync(0xffffffffu, dn, 8 * c) : 1.f;
-      down[t][1] = BF ? __shfl_sync(0xffffffffu, dn, 8 * c + 4) : 1.f;
+        for (int j = 0; j < 4; ++j)
+          xr[hh][j][t] = HALF && !wide ? scaled_pairs(xr[hh][j][t], up) : pair_order(xr[hh][j][t]);
+      down[t][0] = HALF ? __shfl_sync(0xffffffffu, dn, 8 * c) : 1.f;
+      down[t][1] = HALF ? __shfl_sync(0xffffffffu, dn, 8 * c + 4) : 1.f;
     }
   } else {
     // a warp per row and slice; 8 columns from word_col(j, c) lie at 16-byte place 4 j + c of their chunk
-    for (int i = warp; i < M * nsl; i += nw) {
-      const int m = i / nsl, sl = i - m * nsl;
-      const int place = lane & 15, ch = 2 * sl + (lane >> 4);
-      const int k = ch * kChunk + word_col<G>(place >> 2, place & 3);
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (k < K) v = *reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k);
-      float up = 1.f;
-      if constexpr (BF) {
-        float mx = x_max<T>(v), dn;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        up = x_up(mx, dn);
-        if (lane == 0) xdown[sl * 8 + m] = dn;
+    auto stage = [&]() {
+      uint32_t lost = 0;
+      for (int i = warp; i < M * nsl; i += nw) {
+        const int m = i / nsl, sl = i - m * nsl;
+        const int place = lane & 15, ch = 2 * sl + (lane >> 4);
+        const int k = ch * kChunk + word_col<G>(place >> 2, place & 3);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (k < K) v = *reinterpret_cast<const uint4*>(x + (int64_t)m * p.ldx + k);
+        float up = 1.f, dn = 1.f;
+        if (HALF && !wide) {
+          Spread sp;
+          sp.take(v);
+          const uint32_t most = __reduce_max_sync(0xffffffffu, sp.largest());
+          lost = below(v, least_bits(most), lost);
+          up = x_up(bf16_value(most), dn);
+        }
+        if (HALF && lane == 0) xdown[sl * 8 + m] = dn;
+        *reinterpret_cast<uint4*>(xs + (int64_t)m * xpitch + ch * kChunk + place * 8) =
+            HALF && !wide ? scaled_pairs(v, up) : pair_order(v);
       }
-      *reinterpret_cast<uint4*>(xs + (int64_t)m * xpitch + ch * kChunk + place * 8) = x_pairs<T>(v, up);
+      return lost & 0x80008000u;
+    };
+    wide = __syncthreads_or(stage());
+    if (wide) {
+      stage();
+      __syncthreads();
     }
-    __syncthreads();
   }
 
   float acc[NM][MT][4];
@@ -386,6 +433,76 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
         for (int e = 0; e < 4; ++e) acc[mtx][t][e] = 0.f;
   };
   clear();
+  auto products = [&](auto type, int u, int sl) {  // slot u with its part of x, weights widened to `type`
+    using W = decltype(type);
+    if constexpr (!XREG) {
+      down[0][0] = HALF && 2 * c < M ? xdown[sl * 8 + 2 * c] : 1.f;
+      down[0][1] = HALF && 2 * c + 1 < M ? xdown[sl * 8 + 2 * c + 1] : 1.f;
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      uint32_t wd[NM][2][4];
+#pragma unroll
+      for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(wd[mtx][h][0]), "=r"(wd[mtx][h][1]), "=r"(wd[mtx][h][2]), "=r"(wd[mtx][h][3])
+                       : "r"((frag ^ (hh << 6)) + (u * NM + mtx) * MAT + h * 1024) : "memory");
+          spread<G>(wd[mtx][h], c);
+        }
+#pragma unroll
+      for (int g = 0; g < GPC; ++g) {
+        float part[NM][MT][4];
+#pragma unroll
+        for (int mtx = 0; mtx < NM; ++mtx)
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[mtx][t][e] = 0.f;
+#pragma unroll
+        for (int jj = 0; jj < WPG; ++jj) {
+          const int j = g * WPG + jj;
+          uint4 b[MT];
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            if constexpr (XREG) {
+              b[t] = xr[hh][j][t];
+            } else {
+              b[t] = make_uint4(0, 0, 0, 0);
+              if (r + 8 * t < M)
+                b[t] = *reinterpret_cast<const uint4*>(xs + (int64_t)(r + 8 * t) * xpitch + sl * kSlice + hh * kChunk + 32 * j + 8 * c);
+            }
+          }
+#pragma unroll
+          for (int mtx = 0; mtx < NM; ++mtx) {
+            uint32_t lo[4], hi[4];
+            nibbles<W>(wd[mtx][0][j], lo);
+            nibbles<W>(wd[mtx][1][j], hi);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint32_t a[4] = {lo[2 * q], hi[2 * q], lo[2 * q + 1], hi[2 * q + 1]};
+#pragma unroll
+              for (int t = 0; t < MT; ++t) Nib<W>::mma(part[mtx][t], a, q ? b[t].z : b[t].x, q ? b[t].w : b[t].y);
+            }
+          }
+        }
+        const int gi = hh * GPC + g;  // the group in the slice: held by lane gi % 4 of the row
+#pragma unroll
+        for (int mtx = 0; mtx < NM; ++mtx) {
+          const float s0 = scale_of<T>(__shfl_sync(0xffffffffu, sv[u][mtx][0][gi / 4], (lane & 28) + gi % 4));
+          const float s1 = scale_of<T>(__shfl_sync(0xffffffffu, sv[u][mtx][1][gi / 4], (lane & 28) + gi % 4));
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float f = XREG || !HALF ? (e < 2 ? s0 : s1) : (e < 2 ? s0 : s1) * down[t][e & 1];
+              acc[mtx][t][e] = fmaf(part[mtx][t][e], f, acc[mtx][t][e]);
+            }
+        }
+      }
+    }
+  };
   int i = 0, done = 0;  // the item's number in its tile, tiles done
   for (int it0 = 0; it0 < total; it0 += D) {
 #pragma unroll
@@ -395,73 +512,10 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
       cp_wait<D - 1>();
       __syncwarp();
       if (sl < nsl) {
-        if constexpr (!XREG) {
-          down[0][0] = BF && 2 * c < M ? xdown[sl * 8 + 2 * c] : 1.f;
-          down[0][1] = BF && 2 * c + 1 < M ? xdown[sl * 8 + 2 * c + 1] : 1.f;
-        }
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          uint32_t wd[NM][2][4];
-#pragma unroll
-          for (int mtx = 0; mtx < NM; ++mtx)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                           : "=r"(wd[mtx][h][0]), "=r"(wd[mtx][h][1]), "=r"(wd[mtx][h][2]), "=r"(wd[mtx][h][3])
-                           : "r"((frag ^ (hh << 6)) + (u * NM + mtx) * MAT + h * 1024) : "memory");
-              spread<G>(wd[mtx][h], c);
-            }
-#pragma unroll
-          for (int g = 0; g < GPC; ++g) {
-            float part[NM][MT][4];
-#pragma unroll
-            for (int mtx = 0; mtx < NM; ++mtx)
-#pragma unroll
-              for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) part[mtx][t][e] = 0.f;
-#pragma unroll
-            for (int jj = 0; jj < WPG; ++jj) {
-              const int j = g * WPG + jj;
-              uint4 b[MT];
-#pragma unroll
-              for (int t = 0; t < MT; ++t) {
-                if constexpr (XREG) {
-                  b[t] = xr[hh][j][t];
-                } else {
-                  b[t] = make_uint4(0, 0, 0, 0);
-                  if (r + 8 * t < M)
-                    b[t] = *reinterpret_cast<const uint4*>(xs + (int64_t)(r + 8 * t) * xpitch + sl * kSlice + hh * kChunk + 32 * j + 8 * c);
-                }
-              }
-#pragma unroll
-              for (int mtx = 0; mtx < NM; ++mtx) {
-                uint32_t lo[4], hi[4];
-                nibbles_h2(wd[mtx][0][j], lo);
-                nibbles_h2(wd[mtx][1][j], hi);
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                  const uint32_t a[4] = {lo[2 * q], hi[2 * q], lo[2 * q + 1], hi[2 * q + 1]};
-#pragma unroll
-                  for (int t = 0; t < MT; ++t) Nib<__half>::mma(part[mtx][t], a, q ? b[t].z : b[t].x, q ? b[t].w : b[t].y);
-                }
-              }
-            }
-            const int gi = hh * GPC + g;  // the group in the slice: held by lane gi % 4 of the row
-#pragma unroll
-            for (int mtx = 0; mtx < NM; ++mtx) {
-              const float s0 = scale_of<T>(__shfl_sync(0xffffffffu, sv[u][mtx][0][gi / 4], (lane & 28) + gi % 4));
-              const float s1 = scale_of<T>(__shfl_sync(0xffffffffu, sv[u][mtx][1][gi / 4], (lane & 28) + gi % 4));
-#pragma unroll
-              for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float f = XREG || !BF ? (e < 2 ? s0 : s1) : (e < 2 ? s0 : s1) * down[t][e & 1];
-                  acc[mtx][t][e] = fmaf(part[mtx][t][e], f, acc[mtx][t][e]);
-                }
-            }
-          }
-        }
+        if (HALF && wide)
+          products(__nv_bfloat16(), u, sl);
+        else
+          products(typename std::conditional<HALF, __half, T>::type(), u, sl);
       }
       __syncwarp();
       load(u);

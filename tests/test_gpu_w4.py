@@ -195,3 +195,54 @@ def test_modules():
         _check_gate(y, x, m.wg, m.sg, m.wu, m.su)
         assert torch.equal(m(x), ffn.down(y))
         _check_linear(lin(h), h, lin.qweight, lin.scale)
+
+
+def _pack(u):
+    return (u[:, 0::2] | (u[:, 1::2] << 4)).contiguous()
+
+
+def _ruled_out(x, w, s, how, big, G):
+    """Columns of x at ``big``, each beside a weight or a scale that is zero."""
+    w, s, x = w.clone(), s.clone(), x.clone()
+    if how == "scales":
+        x[:, :G] = big  # a whole group, in every chunk of columns
+        s[:, 0] = 0
+        x[:, -G:] = -big
+        s[:, -1] = 0
+    else:
+        u = torch.stack((w & 15, w >> 4), -1).view(w.shape[0], -1)
+        u[:, 5::37] = 8
+        x[:, 5::37] = big
+        w = _pack(u)
+    return x, w, s
+
+
+@pytest.mark.parametrize("how", ["scales", "weights"])
+@pytest.mark.parametrize("big", [2.0 ** 60, 2.0 ** 31 * 1.9921875, 2.0 ** 32, 2.0 ** 100])
+@pytest.mark.parametrize("M,K", [(1, 512), (3, 5120), (8, 1024), (8, 5120), (16, 512), (17, 512), (40, 512), (64, 5120)])
+def test_large_columns_at_zero_weights_change_nothing(M, K, how, big):
+    """Beside columns whose weights are zero the others' products keep every
+    bit: the bound counts no mass for them.  (2^31 and a little: the widest
+    spread that fp16 still holds for 8-bit values; 2^32: the next one.)"""
+    from llms_b200.kernels import int4_fused_gate_up_silu, int4_linear
+    G = 64
+    x = torch.randint(128, 256, (M, K), device="cuda", generator=torch.Generator(device="cuda").manual_seed(M + K)) / 128
+    x[:, 1::2] *= -1
+    x = x.to(BF)
+    x, w, s = _ruled_out(x, *_weights(70, K, G, BF, seed=K), how, big, G)
+    _check_linear(int4_linear(x, w, s), x, w, s)
+    s = s * 2.0 ** -8
+    _check_gate(int4_fused_gate_up_silu(x, w, s, w.flip(0).contiguous(), s.flip(0).contiguous()), x, w, s, w.flip(0), s.flip(0))
+
+
+@pytest.mark.parametrize("M,K", [(1, 256), (8, 256), (2, 5120), (12, 256)])
+def test_x_below_the_normal_numbers(M, K):
+    """All of x subnormal, and subnormal columns beside normal ones whose weights are zero."""
+    from llms_b200.kernels import int4_linear
+    w, s = _weights(40, K, 32, BF, seed=1)
+    s = s * 2.0 ** 40
+    x = (torch.randint(-127, 128, (M, K), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 2.0 ** -133).to(BF)
+    assert x.abs().max() < 2.0 ** -126 and x.any()
+    _check_linear(int4_linear(x, w, s), x, w, s)
+    x, w, s = _ruled_out(x, w, s, "weights", 1.0, 32)
+    _check_linear(int4_linear(x, w, s), x, w, s)
