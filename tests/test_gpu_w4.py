@@ -246,3 +246,39 @@ def test_x_below_the_normal_numbers(M, K):
     _check_linear(int4_linear(x, w, s), x, w, s)
     x, w, s = _ruled_out(x, w, s, "weights", 1.0, 32)
     _check_linear(int4_linear(x, w, s), x, w, s)
+
+
+# K, the most rows of a launch of the stream kernel there (plain, gate-up), and N of a few
+# tiles with a ragged end, and of more tiles than SMs
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("K,G", [(4128, 32), (5120, 64), (5120, 128), (8192, 128), (9728, 32), (9728, 128), (12288, 64), (12288, 128)])
+@pytest.mark.parametrize("M", [1, 3, 4, 6, 8, 9, 16, 17, 33, 64])
+def test_deep_columns(M, K, G, dtype):
+    """Beyond 4096 columns x lies in shared memory where it fits and the warps
+    take several slices; other rows go to the cluster kernel, deep ones in several launches."""
+    from llms_b200.kernels import int4_fused_gate_up_silu, int4_linear
+    N = 2500 if M in (3, 8, 33) else 70
+    x, (w, s) = _x(M, K, dtype), _weights(N, K, G, dtype, seed=M)
+    _check_linear(int4_linear(x, w, s), x, w, s)
+    wu, su = _weights(N, K, G, dtype, seed=M + 1)
+    x = x * 0.1
+    _check_gate(int4_fused_gate_up_silu(x, w, s, wu, su), x, w, s, wu, su)
+
+
+def test_launches_of_one_call_write_their_own_rows_only():
+    """64 rows at 12288 columns take two launches (gate-up four): rows behind the last, and between
+    rows of y, stay; a call of the same rows one launch at a time gives the same bits."""
+    from llms_b200 import _capi
+    from llms_b200.kernels import int4_fused_gate_up_silu, int4_linear
+    M, N, K, G = 50, 130, 12288, 128
+    x, (w, s), (wu, su) = _x(M, K, BF), _weights(N, K, G, BF), _weights(N, K, G, BF, seed=1)
+    y = torch.full((M + 2, 160), 7.0, dtype=BF, device="cuda")
+    st = _capi.lib.b200mm_linear_w4(x.data_ptr(), K, w.data_ptr(), K // 2, s.data_ptr(), K // G, G, y.data_ptr(), 160, M, N, K, 2,
+                                    None, 0, _capi.stream_of(x))
+    assert st == 0 and (y[:, N:] == 7).all() and (y[M:] == 7).all()
+    _check_linear(y[:M, :N].contiguous(), x, w, s)
+    assert torch.equal(y[:32, :N], int4_linear(x[:32], w, s)) and torch.equal(y[32:M, :N], int4_linear(x[32:], w, s))
+    h = x * 0.1
+    g = int4_fused_gate_up_silu(h, w, s, wu, su)
+    for a in range(0, M - 16, 16):
+        assert torch.equal(g[a:a + 16], int4_fused_gate_up_silu(h[a:a + 16], w, s, wu, su))
