@@ -54,12 +54,6 @@ __device__ __forceinline__ float key_value(uint64_t k) {
   return __uint_as_float((b & 0x80000000u) ? b ^ 0x80000000u : ~b);  // (NaN's key reads as a NaN)
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 struct Sums {
   float m, l, e;  // e: of (x - m) log2(e)
 };

@@ -82,10 +82,7 @@ template <> struct Nib<__half> {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   __device__ __forceinline__ static void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    mma_h(d, a[0], a[1], a[2], a[3], b0, b1);
   }
 };
 
@@ -137,21 +134,13 @@ __device__ __forceinline__ void spread(uint32_t (&w)[4], int c) {
 constexpr int kStreamWarps = 16;    // at most
 constexpr int kSlice = 2 * kChunk;  // columns per warp and step: 128 bytes of a row
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {  // zeros where not ok
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Ring slots per warp (2 KB of each matrix a slot).
 __host__ __device__ constexpr int stream_depth(bool gate, bool xreg) { return (xreg ? 6 : 4) / (gate ? 2 : 1); }
 
 // The eight weights of a word as four pairs, (0, 4), (1, 5), (2, 6), (3, 7).  fp16:
 // under the exponent of 2^10 a low half is 1024 + u, a high half 1024 + 16 u, so
-// one shift serves two logic instructions (bf16's 7 bits want one each).
+// one shift serves two logic instructions (bf16's 7 bits want one each).  The way is
+// that of Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't Run" (2022).
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
   uint32_t v;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(mask), "r"(bits));
@@ -294,8 +283,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) w4_stream_kernel(const _
           for (int h = 0; h < 2; ++h) {
             const uint8_t* src = wsrc[mtx] + (h ? 8 * p.ldw : 0);
             const uint32_t dst = frag + (u * NM + mtx) * MAT + h * 1024;
-            cp_async16(dst, src, true);
-            cp_async16(dst ^ 64, src + 64, true);
+            cp_async16(dst, src);
+            cp_async16(dst ^ 64, src + 64);
 #pragma unroll
             for (int q = 0; q < SPL; ++q) sv[u][mtx][h][q] = raw(ssrc[mtx] + (h ? 8 * p.lds : 0) + 4 * q);
           }
