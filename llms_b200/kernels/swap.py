@@ -13,7 +13,7 @@ from torch import nn
 
 from .fused_ffn import TritonFFN
 from .fused_qkv import TritonAttention, triton_fused_qkv
-from .int4 import Int4Attention, Int4FFN, Int4Linear, int4_fused_qkv
+from .int4 import GROUPS, Int4Attention, Int4FFN, Int4Linear, int4_fused_qkv
 from .linear import B200Linear, Int8Linear
 from .quant import Int8Attention, Int8FFN, int8_fused_qkv
 
@@ -48,17 +48,37 @@ def apply_int4_kernels(model: nn.Module, *, group: int = 128, ffn: bool = True, 
     columns and swap in :class:`Int4FFN` / :class:`Int4Attention`, with
     :class:`Int4Linear` for ``attn.o`` / ``ffn.down`` (and, with ``lm_head=True``,
     the LM head).  Modules that hold 8- or 4-bit weights already stay
-    (idempotent; returns ``model``)."""
+    (idempotent; returns ``model``).  A ``group`` that does not divide a
+    projection's columns is refused before anything is swapped.  Up to 16 rows
+    the 4-bit projections are faster than the 16-bit ones, from about 17 on slower."""
+    def dense(lin):
+        if getattr(lin, "bias", None) is not None:
+            raise ValueError("Int4Linear serves bias-free projections only")
+        return isinstance(lin, (nn.Linear, B200Linear))
+
+    def in_features(block):
+        if ffn and not isinstance(block.ffn, (Int8FFN, Int4FFN)):
+            yield block.ffn.gate.weight.shape[1]
+        if qkv and (hasattr(block.attn, "v") or hasattr(block.attn, "W_qkv")):
+            yield (block.attn.W_qkv if hasattr(block.attn, "W_qkv") else block.attn.v.weight).shape[1]
+        for wanted, lin in ((o, block.attn.o), (down, block.ffn.down)):
+            if wanted and dense(lin):
+                yield lin.weight.shape[1]
+
+    head = lm_head and dense(getattr(model, "lm_head", None))
+    for K in [K for block in model.layers for K in in_features(block)] + ([model.lm_head.weight.shape[1]] if head else []):
+        if group not in GROUPS or K % group:  # before the first module is swapped
+            raise ValueError(f"group must be one of {GROUPS} and divide every projection's columns ({K} here), got {group}")
     for block in model.layers:
         if ffn and not isinstance(block.ffn, (Int8FFN, Int4FFN)):
             block.ffn = Int4FFN.from_eager(block.ffn, group=group)
         if qkv and (hasattr(block.attn, "v") or hasattr(block.attn, "W_qkv")):
             block.attn = Int4Attention.from_eager(block.attn, group=group)
-        if o and isinstance(block.attn.o, (nn.Linear, B200Linear)):
+        if o and dense(block.attn.o):
             block.attn.o = Int4Linear.from_linear(block.attn.o, group=group)
-        if down and isinstance(block.ffn.down, (nn.Linear, B200Linear)):
+        if down and dense(block.ffn.down):
             block.ffn.down = Int4Linear.from_linear(block.ffn.down, group=group)
-    if lm_head and isinstance(getattr(model, "lm_head", None), (nn.Linear, B200Linear)):
+    if head:
         model.lm_head = Int4Linear.from_linear(model.lm_head, group=group)
     return model
 

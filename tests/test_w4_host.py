@@ -125,3 +125,21 @@ def test_4_bit_models_are_not_sharded():
     for m in (apply_int4_kernels(Qwen3Model(shape)), apply_int4_kernels(apply_int8_kernels(Qwen3Model(shape)), o=False)):
         with pytest.raises(ValueError, match="4-bit"):
             shard_decode_model(m, 0, 1)
+
+
+@pytest.mark.parametrize("hidden,heads,inter,head_dim,lm_head,group", [(128, 2, 160, 64, False, 128), (128, 2, 256, 48, False, 64), (192, 1, 256, 128, False, 128),
+                                                                       (128, 2, 256, 64, True, 48)])
+def test_a_refused_swap_changes_nothing(hidden, heads, inter, head_dim, lm_head, group):
+    """Columns that the group does not divide, in a projection that comes after others."""
+    from llms_b200.kernels import apply_int4_kernels
+    from llms_b200.qwen3 import Qwen3Model, Qwen3Shape
+    m = Qwen3Model(Qwen3Shape(vocab_size=64, hidden_size=hidden, num_hidden_layers=2, num_attention_heads=heads, num_key_value_heads=1,
+                              head_dim=head_dim, intermediate_size=inter, max_position_embeddings=32))
+    kinds = [type(x) for x in m.modules()]
+    with pytest.raises(ValueError, match="group"):
+        apply_int4_kernels(m, group=group, lm_head=lm_head)
+    assert [type(x) for x in m.modules()] == kinds
+    m.layers[1].attn.o = nn.Linear(heads * head_dim, hidden)
+    with pytest.raises(ValueError):
+        apply_int4_kernels(m, group=32, lm_head=lm_head)
+    assert [type(x) for x in m.modules()] == kinds
