@@ -23,13 +23,11 @@
 //     into [2^14, 2^15): bf16 -> fp16 is then exact to 2^-38 of that element;
 //   * the softmax is local to a block: p = 2^(s - max of the block + 14), held
 //     as two fp16 numbers, p rounded and what that left (22 bits; 2^-39 of the
-//     block's largest still counts), each with its own matrix instruction into
-//     the block's O in fp32, which is joined to the running sums with one factor
-//     that also carries the block's scale of V.  (p in one fp16 number would cost the
-//     outputs as much as their own rounding to fp16 does: with it a norm of 2.5e-4
-//     off the formula instead of 2.1e-4, of which 2.1e-4 are the outputs' rounding.
-//     The second number costs 2 to 4 % of a step that the stream does not bound, 1 x
-//     16384 20.1 -> 20.7 us, and nothing at 16 x 32768.)
+//     block's largest still counts).  Both multiply V into the block's O in fp32,
+//     which is joined to the running sums with one factor that also carries the
+//     block's scale of V.  (p in one fp16 number would cost fp16 outputs nearly as
+//     much as their own rounding does: 2.6e-4 off the formula, by the norm, where the
+//     rounding alone is 2.1e-4.)
 // Each warp has one partial (max, sum, O) per (row, head) that its range touches.
 // Those of a CTA's warps that end in the same pair are joined in shared memory
 // (one long row of 8 KV heads: 18 partials per pair instead of 148 + 18), and a
@@ -150,7 +148,11 @@ struct Seg {
 // rows of 32768: 181 us a step, 172 with twelve).
 __host__ __device__ constexpr int split_warps(int NH) { return NH == 1 ? 12 : 8; }
 
-template <typename T, int D, int NH>
+// SPARE (up to four heads): columns 4..7 are heads 0..3 again, and where the others
+// take p, rounded, they take what that left, so the second number costs no matrix
+// instruction of its own (attention over 1 x 32768: 24.2 us with one, 23.4 so, 23.0
+// without the second number; 32 x 4096 ragged 38.2, 37.7 and 37.3).
+template <typename T, int D, int NH, bool SPARE>
 __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kWarps = split_warps(NH), kThreads = 32 * kWarps;
   constexpr int J = D / 64;             // 16-byte chunks of a K row per lane
@@ -240,6 +242,11 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
   float o[NH][MT][4];
   float m[NH][2], l[NH][2];  // max and this lane's sum, heads 2c, 2c + 1
   auto end_pair = [&](float* acc, float* ml) {  // the partial of the pair: [g][D], [g][2]
+    if constexpr (SPARE)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][i][e] += __shfl_xor_sync(0xffffffffu, o[0][i][e], 2);
 #pragma unroll
     for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -340,7 +347,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
   auto begin_pair = [&](const Seg& s) {
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
-      const int h = 8 * n + r;
+      const int h = SPARE ? r & 3 : 8 * n + r;
       const T* qp = static_cast<const T*>(a.q) + (int64_t)s.b * a.q_sb + ((int64_t)s.kvh * a.g + h) * a.q_sh + 16 * c;
       float f[J][16];
       float mx = 0.f;
@@ -438,7 +445,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
           for (int e = 0; e < 4; ++e)
             if (s < cur.s0 || s >= cur.s1 || 16 * s + r + 8 * (e >> 1) >= cur.valid) sc[n][s][e] = -INFINITY;
     }
-    uint32_t pf[NH][4][2], pr[NH][4][2];  // p in fp16, and what the rounding left, in fp16 too
+    uint32_t pf[NH][4][2], pr[NH][SPARE ? 1 : 4][2];  // p in fp16, and what the rounding left, in fp16 too
     float fo[NH][2], fb[NH][2];  // factors of the running and of the block's sums
     bool same = true;            // no maximum moved
 #pragma unroll
@@ -477,8 +484,9 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
         for (int e = 0; e < 2; ++e) {  // tokens 2c, 2c + 1 of head r, tokens 2c + 8, 2c + 9
           const uint32_t h = pack_h2(p[2 * e], p[2 * e + 1]);
           const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-          pf[n][s][e] = transpose8x8(h);
-          pr[n][s][e] = transpose8x8(pack_h2(p[2 * e] - f.x, p[2 * e + 1] - f.y));
+          const uint32_t left = pack_h2(p[2 * e] - f.x, p[2 * e + 1] - f.y);
+          pf[n][s][e] = transpose8x8(SPARE && c >= 2 ? left : h);
+          if constexpr (!SPARE) pr[n][s][e] = transpose8x8(left);
         }
       }
 #pragma unroll
@@ -526,7 +534,7 @@ __global__ void __launch_bounds__(32 * split_warps(NH), 1) kv8_split_kernel(cons
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
               mma_h(ob[n][i], a0, a1, a2, a3, pf[n][s][0], pf[n][s][1]);
-              mma_h(ob[n][i], a0, a1, a2, a3, pr[n][s][0], pr[n][s][1]);
+              if constexpr (!SPARE) mma_h(ob[n][i], a0, a1, a2, a3, pr[n][s][0], pr[n][s][1]);
             }
           }
         }
@@ -773,10 +781,10 @@ int split_ctas(const b200mm_kv8& c, int rows, int cw) {
   return (int)(need < sms ? need : sms);
 }
 
-template <typename T, int D, int NH>
+template <typename T, int D, int NH, bool SPARE>
 int run_fast(const AttnArgs& a, cudaStream_t st) {
   constexpr size_t smem = (size_t)split_warps(NH) * 2 * 64 * D;
-  auto kern = kv8_split_kernel<T, D, NH>;
+  auto kern = kv8_split_kernel<T, D, NH, SPARE>;
   const int dev = current_device();
   static bool configured[64] = {false};
   if (dev < 0 || dev >= 64) return B200MM_ERR_DEVICE;
@@ -795,8 +803,11 @@ template <typename T>
 int run(const AttnArgs& a, bool fast, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
     if (fast) {
-      if (a.c.D == 128) return a.g <= 8 ? run_fast<T, 128, 1>(a, st) : run_fast<T, 128, 2>(a, st);
-      return a.g <= 8 ? run_fast<T, 64, 1>(a, st) : run_fast<T, 64, 2>(a, st);
+      if (a.c.D == 128)
+        return a.g <= 4 ? run_fast<T, 128, 1, true>(a, st)
+               : a.g <= 8 ? run_fast<T, 128, 1, false>(a, st) : run_fast<T, 128, 2, false>(a, st);
+      return a.g <= 4 ? run_fast<T, 64, 1, true>(a, st)
+             : a.g <= 8 ? run_fast<T, 64, 1, false>(a, st) : run_fast<T, 64, 2, false>(a, st);
     }
   }
   return launch_pdl(kv8_generic_kernel<T>, dim3(a.H, a.B), dim3(kGenericThreads), 0, st, a) == cudaSuccess
