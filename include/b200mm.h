@@ -141,11 +141,12 @@ int b200mm_qkv_w8(const void* x, int64_t ldx,
  *       2 i + 1 in the high half of byte i; 16-byte aligned (address and stride)
  *   s : `dtype` [N, K / group], row stride lds
  *   x, y : `dtype` (F16 or BF16); x 16-byte aligned (address and row stride)
- * K is a multiple of group and at most 65536, N at most 2^24.  y = x W^T, fp32 accumulation, no product rounded;
- * the gate/up variant y = silu(x Wg^T) * (x Wu^T).  From M = 65 on the
+ * K is a multiple of group and at most 65536, N at most 2^24.  y = x W^T, fp32 accumulation, no product rounded
+ * (a group's x u are summed before its scale: |x| below 2^118 keeps that sum
+ * finite); the gate/up variant y = silu(x Wg^T) * (x Wu^T).  From M = 65 on the
  * weights are first expanded to `dtype` (rounded once) into the workspace:
- * b200mm_w4_workspace_size bytes (0 below that), 256-byte aligned, owned by
- * the stream until the call completes.
+ * b200mm_w4_workspace_size bytes (2 per weight and 16 more; 0 below that),
+ * 256-byte aligned, owned by the stream until the call completes.
  */
 size_t b200mm_w4_workspace_size(int64_t M, int64_t N, int64_t K, int gate);
 

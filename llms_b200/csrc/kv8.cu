@@ -23,9 +23,11 @@
 // from the tail) and write one row of 8 bits while the scale stands.
 // expand: 16 values per thread.
 // Measured (B200, bf16, KV 8, D 128): 4096 tokens of one row in 9.3 us (25 MB moved,
-// 2.7 TB/s; 8 MB of it stay in L2) and out in 7.1 us, 4 x 1537 in 13.5 and 9.1.  The
-// append is bound by integer instructions (the maximum, the packing, the test for a
-// border: issue 66 %, special-function pipe 5 %), the expansion by the stream.
+// 2.7 TB/s; 8 MB of it stay in L2) and out in 7.0 us (3.6 TB/s), 4 x 1537 in 13.5 and
+// 9.2; 3.8 us would be the copy rate.  Most of the append is integer instructions (the
+// maximum, the packing, the test for a border: issue 66 %, special-function pipe 5 %) and
+// its CTAs' waits for load, maximum and store in turn; the expansion has two loads a
+// thread in flight and a division for each.
 #include "kv8.cuh"
 
 namespace b200mm {

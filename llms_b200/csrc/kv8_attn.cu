@@ -30,17 +30,18 @@
 //     rounding alone is 2.1e-4.)
 // Each warp has one partial (max, sum, O) per (row, head) that its range touches.
 // Those of a CTA's warps that end in the same pair are joined in shared memory
-// (one long row of 8 KV heads: 18 partials per pair instead of 148 + 18), and a
+// (one long row of 8 KV heads: the 222 warps of a pair leave 19 or 20), and a
 // second kernel joins the rest.
 //
-// Measured (B200, bf16, H 32, KV 8, D 128): 16 rows of 32768 tokens 166-174 us, 6.2
-// to 6.5 TB/s of cache; 32 rows of 4096 52 us (5.2 TB/s), of 1..4096 at random 32 us
-// (4.1); 1 row of 32768 22 us (3.0), of 512 8.6 us; the append adds 2 to 6 us to a step
-// (it runs beside the attention, but its CTAs and the attention's do not fit on
-// one SM).  Long contexts are bound by HBM (at 16 x 32768 the schedulers issue in 64 %
-// of the cycles, so not by much); short ones by what does not shrink: two dependent
-// launches, the plan, one block's latency and the joins, 8 us; those between
-// by whole blocks per warp (1 x 32768: 4096 blocks for 1776 warps, three rounds).
+// Measured (B200, bf16, H 32, KV 8, D 128; attention, and the step with its append):
+// 16 rows of 32768 tokens 165 us, 6.5 TB/s of cache, 171-178 the step; 32 rows of 4096
+// 52.6 us (5.1 TB/s) and 58, of 1..4096 at random 37.7 (3.9) and 42; 1 row of 32768
+// 23.4 (2.9) and 26.8, of 512 8.9 and 11.5 (the append runs beside the attention, but
+// its CTAs and the attention's do not fit on one SM).  Long contexts are bound by HBM (at
+// 16 x 32768 the schedulers issue in 66 % of the cycles, so not by much); short ones by
+// what does not shrink: two dependent launches, the plan, one block's latency and the
+// joins, 8 us; those between by whole blocks per warp (1 x 32768: 4096 blocks for 1776
+// warps, three rounds).
 //
 // Other shapes (fp32, head dims other than 64 / 128, more than 16 query heads
 // per KV head) run a kernel of one CTA per (head, row) on plain arithmetic.

@@ -17,22 +17,27 @@
 //   * a group's products are summed in fp32 in accumulators of their own, which
 //     its scale then joins to the row's: no product is rounded;
 //   * before griddepcontrol.wait a CTA only asks for its first weights in L2.
-// Up to 16 rows of x, one persistent CTA per SM walks tiles of 16 weight rows.
-// Its warps split K; each has the part of x that it needs in registers (or, for
-// long K, x lies in shared memory) and fills a ring of its own with cp.async,
-// several tiles ahead, so only the sums of a tile meet at a barrier.  Otherwise K
-// is split over a cluster of CTAs with 128 weight rows each, and the sums meet in
-// distributed shared memory (12288 x 4096 gate and up: one row 25 us there and 16 in the
-// persistent kernel, 16 rows 50 and 28).
+// Up to 16 rows of x and 4096 columns, one persistent CTA per SM walks tiles of 16
+// weight rows.  Its warps split K; each has the part of x that it needs in registers
+// and fills a ring of its own with cp.async, several tiles ahead, so only the sums
+// of a tile meet at a barrier.  With more columns x lies in shared memory, where up to 8
+// rows of it fit beside the rings (stream_fits: 8 rows at 5120 columns, 5 at 8192, 3 at
+// 12288).  Otherwise K is split over a cluster of CTAs with 128 weight rows each, and
+// the sums meet in distributed shared memory (12288 x 4096 gate and up: one row 25 us
+// there and 16 in the persistent kernel, 16 rows 50 and 28; 4096 x 12288: 3 rows 14.5
+// us here, 4 to 8 rows 16.5 there; 4096 x 8192: 5 rows 12.4, 6 to 8 rows 12.3), as many
+// rows of x a launch as shared memory takes (rows_per_launch), each launch reading
+// all weights: 4096 x 12288 26.6 us at 32 rows, 52 at 64 in two launches.
 // From kDenseRows on the weights are expanded to 16 bits (rounded once: the
 // tcgen05 GEMM's operands are 16-bit) into the caller's workspace and the dense
-// GEMM takes them.  12288 x 4096 gate and up: 113 us at 128 rows, where two launches
+// GEMM takes them.  12288 x 4096 gate and up: 114 us at 128 rows, where two launches
 // of 64 take 165; 83 us at 64 rows, where this would take 127 (65 to 80 rows would
 // still be 100 to 112 in two launches, but 4096 x 12288 69 to 84 instead of 66).
-// Measured (cold weights, G = 128): 12288 x 4096 gate and up 15-16 us at one row (3.4
-// TB/s), 18 at 8, 28 at 16, 46 at 32; 6144 x 4096 6.1 us at one row, 10.9 at 16.  Not
-// HBM bounds these but instructions: issue slots half full, no pipe full, four warps
-// per scheduler.
+// Measured (weights rotated past L2, G = 128): 12288 x 4096 gate and up 16.6 us at one
+// row (3.1 TB/s), 19.0 at 8, 28.8 at 16, 47 at 32; 6144 x 4096 6.4-6.9 us at one row,
+// 10.7 at 16.  Not HBM bounds these but instructions and fetching them: issue slots
+// half full, no pipe full, four warps per scheduler.  (From 17 rows on the dense
+// projections with 16-bit weights are as fast, 45 us there, and at 64 rows faster, 50.)
 #include "w4.cuh"
 
 #include <type_traits>
