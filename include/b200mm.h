@@ -248,7 +248,8 @@ int b200mm_gqa_decode(const void* q, int64_t q_sb, int64_t q_sh,
  *   S - 1), g = H / KV; zeros where p is negative.  q, out: [B, H, D] `dtype`;
  *   q 16-byte aligned (address and strides).  fp32 softmax and accumulation,
  *   16-bit products (exact for the 8-bit values; a probability is the sum of two
- *   16-bit numbers and keeps 22 bits), one rounding on store.  16-bit types with D = 64 or 128 and g <= 16
+ *   16-bit numbers and keeps 22 bits; a bf16 query enters within 2^-38 of its
+ *   head's largest element), one rounding on store.  16-bit types with D = 64 or 128 and g <= 16
  *   take the split-context kernel; everything else a generic kernel.
  *   workspace: >= b200mm_kv8_decode_workspace_size bytes (may be 0), 256-byte
  *   aligned, owned by the stream until the call completes; nothing in it has
